@@ -305,6 +305,108 @@ PXB_API int pxb_batched_update(int64_t cap, const int32_t *from_id,
                        float *opt_t, void *stream);
 
 /* ------------------------------------------------------------------ */
+/* microscaled (MX) unit rows and the edge products that read them     */
+/* ------------------------------------------------------------------ */
+
+/* A row of `batch` samples of one unit is ceil(batch / 32) blocks. A block is
+ * one scale byte (2^(byte - 127); 255: the block is not a number) and 32
+ * codes: 32 bytes of e4m3 or e5m2, or 16 bytes of e2m1 (the even sample in
+ * the low nibble). Rows of codes are [num_units, blocks * 32 or 16] bytes,
+ * 16-byte aligned; rows of scales [num_units, blocks] bytes. The samples past
+ * `batch` in the last block are code 0.
+ * Quantisation: the scale is the smallest power of two s (at least 2^-127)
+ * with max|x| <= s * (the format's largest value); a code is x / s rounded to
+ * the nearest element, ties to even. A block with an infinity or a NaN takes
+ * the scale 255. `keep_nonzero`: a value other than 0 that would round to 0
+ * takes the smallest magnitude of its sign instead. */
+#define PXB_MX_E4M3 0
+#define PXB_MX_E5M2 1
+#define PXB_MX_E2M1 2
+#define PXB_MX_F32 3 /* not microscaled: float32 values */
+
+#define PXB_DT_F32 0
+#define PXB_DT_BF16 1
+#define PXB_DT_F16 2
+
+/* Row i of x (element b at x + i * stride_row + b * stride_sample, in
+ * elements of `dtype`) into row ids[i] (NULL: row i) of codes / scales. An id
+ * outside [0, num_units) is skipped; other rows stay as they were. */
+PXB_API int pxb_mx_quantize(int32_t num_rows, int32_t batch, const void *x,
+                            int32_t dtype, int64_t stride_row,
+                            int64_t stride_sample, int32_t fmt,
+                            int32_t keep_nonzero, const int64_t *ids,
+                            int32_t num_units, uint8_t *codes,
+                            uint8_t *scales, void *stream);
+/* out[u * ld + b] = the values of the rows. */
+PXB_API int pxb_mx_dequantize(int32_t num_units, int32_t batch,
+                              const uint8_t *codes, const uint8_t *scales,
+                              int32_t fmt, void *out, int32_t dtype,
+                              int64_t ld, void *stream);
+/* The batched forward's apply with its checkpoint, over [N, B] float32 rows:
+ * for the units with level == target_level (level NULL: all), rows = act(rows)
+ * in place (a unit of role 1 keeps its row) and the result's codes with
+ * keep_nonzero, e4m3 or e5m2. Replaces pxb_batched_unit_apply mode 0 when the
+ * backward reads a checkpoint. */
+PXB_API int pxb_mx_unit_apply(int32_t num_units, int32_t batch,
+                              int32_t act_kind, float *rows,
+                              const int32_t *level, int32_t target_level,
+                              const uint8_t *roles, int32_t fmt,
+                              uint8_t *codes, uint8_t *scales, void *stream);
+/* out = (acc + seed) * act'(a) with the derivative taken from the activations
+ * a of a checkpoint, over [N, B] float32 rows (seed NULL: none); rows masked
+ * by level and role 1 are left. `out` may be `acc`. Stands in for
+ * pxb_batched_unit_apply mode 1. */
+PXB_API int pxb_mx_unit_grad(int32_t num_units, int32_t batch,
+                             int32_t act_kind, const float *acc,
+                             const float *seed, const uint8_t *codes,
+                             const uint8_t *scales, int32_t fmt,
+                             const int32_t *level, int32_t target_level,
+                             const uint8_t *roles, float *out, void *stream);
+/* The batch-mean gradient of every slot from checkpointed activations a:
+ *   stat[s] = (sum_b g[to[s], b] * a[from[s], b]) / B   for live s,
+ * summed in float32. With opt NULL, dw[s] = stat (0 for a dead slot, or one
+ * whose ids are out of range); otherwise one optimizer step as
+ * pxb_batched_update (dw must be NULL). Any batch >= 1. */
+PXB_API int pxb_mx_edge_grad(int64_t cap, const int32_t *from_id,
+                             const int32_t *to_id, const uint8_t *dead,
+                             const float *g, const uint8_t *codes,
+                             const uint8_t *scales, int32_t fmt, int32_t batch,
+                             int32_t num_units, float *dw, float *weight,
+                             const pxb_optimizer *opt, float *opt_m,
+                             float *opt_v, float *opt_t, void *stream);
+
+/* In-edges grouped by destination: edges [offsets[i], offsets[i + 1]) of
+ * `src` end in unit units[i]. Weights are float32 (fmt PXB_MX_F32: `weight`,
+ * one an edge) or MX blocks of 32 consecutive in-edges of one destination:
+ * blocks [block_offsets[i], block_offsets[i + 1]) of `codes` / `scales`. */
+typedef struct pxb_mx_conns {
+  int32_t num_dst;
+  int32_t fmt;
+  int64_t num_edges;  /* of src (and weight): no edge past it is read */
+  int64_t num_blocks; /* of scales: no block past it is read */
+  const int32_t *units;
+  const int64_t *offsets;
+  const int32_t *src;
+  const float *weight;
+  const int64_t *block_offsets;
+  const uint8_t *codes;
+  const uint8_t *scales;
+} pxb_mx_conns;
+
+/* out[units[i], b] = act(sum_e w[e] * x[src[e], b]), summed in float32, for
+ * every i (act(0) where a destination has no edges); other rows of out stay
+ * as they were. x is float32 [num_src, B] or MX rows; out float32 [num_out, B]
+ * or MX rows (quantised from the float32 result). An edge whose source is
+ * outside [0, num_src) and a unit outside [0, num_out) are skipped. x and out
+ * may be one buffer where no destination is a source. */
+PXB_API int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src,
+                           int32_t batch, const float *x,
+                           const uint8_t *x_codes, const uint8_t *x_scales,
+                           int32_t x_fmt, int32_t act_kind, int32_t num_out,
+                           float *out, uint8_t *out_codes,
+                           uint8_t *out_scales, int32_t out_fmt, void *stream);
+
+/* ------------------------------------------------------------------ */
 /* growth                                                              */
 /* ------------------------------------------------------------------ */
 

@@ -14,6 +14,18 @@ from plastax_b200.builder import NetworkBuilder
 from plastax_b200.state import NetworkState, NetworkStatic, live_conn_count, make_empty_state
 from plastax_b200.state import grow_bucket
 from plastax_b200.driver import Driver
+from plastax_b200.infer import InferFn, make_infer
+from plastax_b200.mx import (
+    MxConns,
+    MxRows,
+    mx_dequantize,
+    mx_edge_grad,
+    mx_product,
+    mx_quantize,
+    mx_unit_apply,
+    mx_unit_grad,
+    mx_update,
+)
 from plastax_b200.step import GrowthRemainder, StepFn, StepInputs, StepResult, make_growth_retry, make_step
 from plastax_b200.shortlist import ShortlistCoverage, recommended_shortlist, shortlist_coverage
 from plastax_b200.topo import resort
@@ -63,6 +75,8 @@ __all__ = [
     "BackwardPass", "DestinationThresholdPrune", "Driver", "FieldSpec", "ForwardPass", "GrowthRemainder", "MSELoss",
     "MagnitudePrune", "MeanFloatFirstRest", "Network", "NetworkBuilder", "NetworkState", "NetworkStatic", "Propagation", "ProposeAddConn",
     "PruneConn", "PxbError", "ResetGlobal", "ScoreAddConn", "ShardSpec", "SoftmaxCrossEntropyLoss", "StepFn", "StepInputs", "StepResult", "live_conn_count",
+    "InferFn", "MxConns", "MxRows", "make_infer", "mx_dequantize", "mx_edge_grad", "mx_product", "mx_quantize",
+    "mx_unit_apply", "mx_unit_grad", "mx_update",
     "grow_bucket", "make_empty_state", "make_growth_retry", "make_step", "monoid", "optim", "predicate_add_conn",
     "recommended_shortlist", "resort", "shortlist_coverage", "ShortlistCoverage",
 ]

@@ -47,6 +47,7 @@ PAIR_ABS_PRODUCT, PAIR_PRODUCT, PAIR_MODULAR, PAIR_MODULAR_PREDICATE = 0, 1, 2, 
 UNIT_UPDATE_AFFINE, UNIT_UPDATE_TRACE_ABS, UNIT_UPDATE_TRACE = 0, 1, 2
 SPAWN_FIELD_AT_LEAST, SPAWN_ARGMAX = 0, 1
 MAX_UNIT_COLUMNS = 16
+MX = {"e4m3": 0, "e5m2": 1, "e2m1": 2, "f32": 3}
 
 
 def act_code(kind) -> int:
@@ -153,6 +154,24 @@ class Optimizer(ctypes.Structure):
         ("eps", c_f32),
         ("weight_decay", c_f32),
         ("unit_scale", c_ptr),
+    ]
+
+
+class MxConns(ctypes.Structure):
+    """`pxb_mx_conns`: in-edges grouped by destination, weights in float32 or MX blocks."""
+
+    _fields_ = [
+        ("num_dst", c_i32),
+        ("fmt", c_i32),
+        ("num_edges", c_i64),
+        ("num_blocks", c_i64),
+        ("units", c_ptr),
+        ("offsets", c_ptr),
+        ("src", c_ptr),
+        ("weight", c_ptr),
+        ("block_offsets", c_ptr),
+        ("codes", c_ptr),
+        ("scales", c_ptr),
     ]
 
 
@@ -322,6 +341,16 @@ _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "pxb_pipeline_train_max_units": (c_i32, [c_i32]),
     "pxb_pipeline_train_scratch_bytes": (c_i32, [c_i32, ctypes.POINTER(c_size)]),
     "pxb_pipeline_train_step": (c_i32, [c_ptr, c_ptr]),
+    "pxb_mx_quantize": (c_i32, [c_i32, c_i32, c_ptr, c_i32, c_i64, c_i64, c_i32, c_i32, c_ptr, c_i32, c_ptr, c_ptr,
+                                c_ptr]),
+    "pxb_mx_dequantize": (c_i32, [c_i32, c_i32, c_ptr, c_ptr, c_i32, c_ptr, c_i32, c_i64, c_ptr]),
+    "pxb_mx_unit_apply": (c_i32, [c_i32, c_i32, c_i32, c_ptr, c_ptr, c_i32, c_ptr, c_i32, c_ptr, c_ptr, c_ptr]),
+    "pxb_mx_unit_grad": (c_i32, [c_i32, c_i32, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_ptr, c_i32, c_ptr, c_ptr,
+                                 c_ptr]),
+    "pxb_mx_edge_grad": (c_i32, [c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_i32, c_i32, c_ptr, c_ptr,
+                                 c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "pxb_mx_product": (c_i32, [c_ptr, c_i32, c_i32, c_ptr, c_ptr, c_ptr, c_i32, c_i32, c_i32, c_ptr, c_ptr, c_ptr,
+                               c_i32, c_ptr]),
     "pxb_propose_grid": (c_i32, [c_i32, c_i32, c_i32, c_i32, c_ptr, c_ptr, c_i32, c_ptr, c_ptr, c_ptr, c_i32, c_i32,
                                  c_i32, c_i32, c_ptr, c_ptr, c_ptr, c_ptr]),
 }

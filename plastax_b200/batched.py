@@ -10,15 +10,29 @@ reduce to the state's columns by the net's `batch_reduction`
 (MeanFloatFirstRest: the batch mean of every float column), and prune and
 growth run once on the reduced state, as the streaming step runs them.
 `StepResult.loss` is the batch mean.
+
+With `activation_checkpoint` ("e4m3" / "e5m2", plastax_b200/mx.py) the backward
+pass and the update read the activations from 8-bit blocks that the forward's
+applies leave behind; the forward and the loss stay in float32. One [N, B]
+float32 buffer then holds, row by row, the forward's sums, the activations
+made from them in place and, once the checkpoint has them, the backward's sums
+and gradients: 4 (rows) + 4 (the loss seeds) + 33/32 bytes a unit and sample
+instead of 16. A row serves all of these because an edge of a TOPOLOGICAL net
+goes to a deeper level, so a level's sums are complete before its apply. The
+step checks a state for that when it first sees it, and the growth rule must
+have direction "deeper".
 """
 
 from __future__ import annotations
+
+import weakref
 
 import numpy as np
 import torch
 
 from plastax_b200 import _lib
 from plastax_b200 import kernels as K
+from plastax_b200 import mx
 from plastax_b200.state import NetworkState, NetworkStatic
 from plastax_b200.step import StepFn, StepInputs, StepResult
 from plastax_b200.traits import (
@@ -36,7 +50,15 @@ class BatchedStepFn:
     """A built batched step: [N, B] unit rows plus a streaming StepFn whose
     structural phases run on the reduced state."""
 
-    def __init__(self, net: type[Network], static: NetworkStatic, batch_size: int, device: torch.device) -> None:
+    def __init__(self, net: type[Network], static: NetworkStatic, batch_size: int, device: torch.device,
+                 activation_checkpoint: str | None = None) -> None:
+        if activation_checkpoint is not None:
+            if activation_checkpoint not in mx.CHECKPOINT_FORMATS:
+                raise ValueError(f"make_step: unknown activation_checkpoint {activation_checkpoint!r}: one of "
+                                 f"{', '.join(mx.CHECKPOINT_FORMATS)}")
+            if net.add_conn is not None and net.add_conn.direction != "deeper":
+                raise NotImplementedError("activation_checkpoint reuses a unit's row once its level is applied: the "
+                                          "growth rule must have direction 'deeper'")
         if batch_size % 4 != 0 or batch_size > 1024:
             raise ValueError(f"make_step: the batched engine moves unit rows as float4: batch_size must be a "
                              f"multiple of 4 and at most 1024, got {batch_size}")
@@ -59,9 +81,17 @@ class BatchedStepFn:
         self.inner.ahead = False  # the structural phases run on the reduced state, in the step
         n, B = static.num_units, self.batch
         z = lambda: torch.zeros((n, B), dtype=torch.float32, device=device)  # noqa: E731
-        self.act_b, self.acc_b = z(), z()
+        self.acc_b = z()
+        self.checkpoint = None  # the activations in 8-bit blocks; rows are then shared (see the module's notes)
+        self._checked_state: weakref.ref | None = None
         bp, loss = net.backward_pass, net.loss
-        self.grad_b = z() if bp is not None else None
+        if activation_checkpoint is not None:
+            self.checkpoint = mx.MxRows.empty(n, B, activation_checkpoint, device, zero=True)
+            self.act_b = self.acc_b
+            self.grad_b = self.acc_b if bp is not None else None
+        else:
+            self.act_b = z()
+            self.grad_b = z() if bp is not None else None
         self.seed_b = z() if loss is not None else None
         self.loss_b = torch.zeros(B, dtype=torch.float32, device=device)
         self.launches = 0
@@ -105,13 +135,68 @@ class BatchedStepFn:
                              free_bitmap=bm, bitmap_level=bm_level)
             self.launches += 1
 
-    def __call__(self, state: NetworkState, inputs: StepInputs) -> StepResult:
+    def _check_deeper(self, state: NetworkState) -> None:
+        """Every live edge goes to a deeper level (once per state; reads the
+        host). Edges into inputs, which sit at level 0, do not."""
+        if self._checked_state is not None and self._checked_state() is state:
+            return
+        level = state.units[LEVEL.name]
+        n = self.static.num_units
+        for i, b in enumerate(state.conns):
+            live = b["dead"] == 0
+            f, t = b["from_id"][live].clamp(0, n - 1).long(), b["to_id"][live].clamp(0, n - 1).long()
+            if bool((level[t] <= level[f]).any()):
+                raise ValueError(f"activation_checkpoint: bucket {i} has an edge that does not go to a deeper level")
+        self._checked_state = weakref.ref(state)
+
+    def _call_checkpointed(self, state: NetworkState, x: torch.Tensor, inputs: StepInputs) -> None:
+        """The propagation and the update of a step whose backward reads the
+        checkpoint; acc_b, act_b and grad_b are one buffer."""
+        net, inner, units, rows, ck = self.net, self.inner, state.units, self.acc_b, self.checkpoint
+        level, roles, L = units[LEVEL.name], inner.is_input, self.num_levels
+        self._check_deeper(state)
+        rows.zero_()
+        rows.index_copy_(0, inner.input_ids, x.t())
+        mx.mx_quantize(x.t(), ck.fmt, keep_nonzero=True, ids=inner.input_ids, out=ck)
+        for lv in range(L):
+            K.batched_forward(state.conns[lv], rows, rows)
+            mx.mx_unit_apply(rows, ck, inner.fwd_act, level=level, target_level=lv + 1, roles=roles)
+        self._loss(inputs)
+        K.batch_mean(rows, units[ACTIVATION.name])
+        bp = net.backward_pass
+        if bp is not None:
+            rows.zero_()
+            mx.mx_unit_grad(rows, ck, inner.bwd_act, seed=self.seed_b, level=level, target_level=L, roles=roles,
+                            out=rows)
+            for lv in range(L - 1, 0, -1):
+                K.batched_backward(state.conns[lv], rows, rows)
+                mx.mx_unit_grad(rows, ck, inner.bwd_act, seed=self.seed_b, level=level, target_level=lv, roles=roles,
+                                out=rows)
+        if net.update_conn is not None:
+            for b in state.conns:
+                mx.mx_update(b, self.upd_grad_b, ck, inner.opt)
+        self.launches += 2 * L + 1 + (0 if bp is None else 2 * L - 1) + (len(state.conns) if net.update_conn else 0)
+
+    def _loss(self, inputs: StepInputs) -> None:
+        """Loss, per sample; the batch mean to StepResult.loss."""
+        loss = self.net.loss
+        if loss is None:
+            return
+        if inputs.targets is None:
+            raise ValueError("a network with a loss needs StepInputs.targets")
+        t = self._rows(inputs.targets, len(self.static.output_ids))
+        kind = _lib.LOSS_SOFTMAX_CE if isinstance(loss, SoftmaxCrossEntropyLoss) else _lib.LOSS_MSE
+        if not isinstance(loss, (MSELoss, SoftmaxCrossEntropyLoss)):
+            raise NotImplementedError(f"loss {type(loss).__name__} has no engine lowering")
+        K.batched_loss(kind, self.inner.output_ids, self.batch, self.act_b, t, self.seed_b, self.loss_b,
+                       self.inner.loss_buf)
+        self.launches += 2
+
+    def _call_plain(self, state: NetworkState, x: torch.Tensor, inputs: StepInputs) -> None:
+        """The propagation and the update of a step on float32 rows."""
         net, inner, units = self.net, self.inner, state.units
-        inner._bind(state)
-        inner._level = units[LEVEL.name]
         level, is_input = units[LEVEL.name], inner.is_input
         L = self.num_levels
-        x = self._rows(inputs.inputs, len(self.static.input_ids))
         self.act_b.index_copy_(0, inner.input_ids, x.t().contiguous())
         # forward, level by level (src/plastax/phases.py:972-1015)
         fp = net.forward_pass
@@ -121,18 +206,7 @@ class BatchedStepFn:
             K.batched_unit_apply(self.acc_b, self.act_b, mode=0, act_kind=inner.fwd_act, level=level,
                                  target_level=lv + 1, is_input=is_input)
             self.launches += 2
-        # loss, per sample; the batch mean to StepResult.loss
-        loss = net.loss
-        if loss is not None:
-            if inputs.targets is None:
-                raise ValueError("a network with a loss needs StepInputs.targets")
-            t = self._rows(inputs.targets, len(self.static.output_ids))
-            kind = _lib.LOSS_SOFTMAX_CE if isinstance(loss, SoftmaxCrossEntropyLoss) else _lib.LOSS_MSE
-            if not isinstance(loss, (MSELoss, SoftmaxCrossEntropyLoss)):
-                raise NotImplementedError(f"loss {type(loss).__name__} has no engine lowering")
-            K.batched_loss(kind, inner.output_ids, self.batch, self.act_b, t, self.seed_b, self.loss_b,
-                           inner.loss_buf)
-            self.launches += 2
+        self._loss(inputs)
         # backward, deepest level first (src/plastax/phases.py:1049-1104)
         bp = net.backward_pass
         if bp is not None:
@@ -149,8 +223,19 @@ class BatchedStepFn:
             for b in state.conns:
                 K.batched_update(b, self.upd_grad_b, self.act_b, inner.opt)
                 self.launches += 1
-        # per-sample unit columns -> the state's (batch_reduction)
         K.batch_mean(self.act_b, units[ACTIVATION.name])
+
+    def __call__(self, state: NetworkState, inputs: StepInputs) -> StepResult:
+        net, inner, units = self.net, self.inner, state.units
+        inner._bind(state)
+        inner._level = units[LEVEL.name]
+        x = self._rows(inputs.inputs, len(self.static.input_ids))
+        if self.checkpoint is not None:
+            self._call_checkpointed(state, x, inputs)
+        else:
+            self._call_plain(state, x, inputs)
+        bp, loss = net.backward_pass, net.loss
+        # per-sample unit columns -> the state's (batch_reduction)
         if bp is not None:
             K.batch_mean(self.grad_b, units[bp.grad_field.name])
         if loss is not None:

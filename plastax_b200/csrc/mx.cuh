@@ -1,0 +1,147 @@
+// Microscaled (MX) values: blocks of 32 that share a power-of-two scale byte
+// (E8M0: 2^(byte - 127), 255 = not a number) with codes in e4m3, e5m2 (one
+// byte each) or e2m1 (two to a byte, the even element in the low nibble).
+//
+// Encoding of a block x_0..x_31: the scale is the smallest power of two s >=
+// 2^-127 with max|x_i| <= L * s (L the format's largest value, so nothing
+// saturates and at most one bit of the range is unused), the code of x_i the
+// nearest element to x_i / s, ties to even. The division is a product with
+// 2^-e, exact down to where the code is 0 anyway. A block that holds an
+// infinity or a NaN gets the scale 255 and reads NaN whole: a partial sum over
+// it is then NaN too, as it would be in float32.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+#include "pxb_common.cuh"
+
+namespace pxb {
+
+constexpr int kMxBlock = 32;
+
+template <int FMT>
+struct MxFormat;
+template <>
+struct MxFormat<PXB_MX_E4M3> {
+  static constexpr int bits = 8, top_exp = 8;
+  static constexpr uint32_t top_mant = 0x600000u;  // 448 = 1.75 * 2^8
+};
+template <>
+struct MxFormat<PXB_MX_E5M2> {
+  static constexpr int bits = 8, top_exp = 15;
+  static constexpr uint32_t top_mant = 0x600000u;  // 57344 = 1.75 * 2^15
+};
+template <>
+struct MxFormat<PXB_MX_E2M1> {
+  static constexpr int bits = 4, top_exp = 2;
+  static constexpr uint32_t top_mant = 0x400000u;  // 6 = 1.5 * 2^2
+};
+
+template <int FMT>
+__host__ __device__ constexpr int mx_block_bytes() {
+  return kMxBlock * MxFormat<FMT>::bits / 8;
+}
+
+__host__ __device__ inline int mx_bits(int fmt) { return fmt == PXB_MX_E2M1 ? 4 : 8; }
+__host__ __device__ inline int64_t mx_blocks(int64_t n) { return (n + kMxBlock - 1) / kMxBlock; }
+
+// The value of a scale byte.
+__device__ __forceinline__ float mx_scale_value(uint32_t s) {
+  return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23);
+}
+
+// The scale byte of a block whose largest magnitude has these bits.
+template <int FMT>
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return 255u;
+  const int e = static_cast<int>(amax_bits >> 23) - MxFormat<FMT>::top_exp +
+                ((amax_bits & 0x7fffffu) > MxFormat<FMT>::top_mant ? 1 : 0);
+  return static_cast<uint32_t>(e < 0 ? 0 : e);
+}
+
+// 2^-e of a scale byte e + 127 (0 for the byte 255, whose codes are all 0).
+__device__ __forceinline__ float mx_inverse_scale(uint32_t s) {
+  return s == 255u ? 0.0f : __uint_as_float((254u - s) << 23);
+}
+
+// Eight consecutive values -> eight codes (8 bytes, or 4 for e2m1), given
+// 2^-e. `keep`: a value that is not zero takes at least the smallest
+// magnitude of its sign, so its sign survives.
+template <int FMT>
+__device__ __forceinline__ uint64_t mx_encode8(const float (&x)[8], uint32_t scale, bool keep) {
+  if (scale == 255u) return 0;
+  const float inv = mx_inverse_scale(scale);
+  uint64_t out = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 y = make_float2(__fmul_rn(x[i], inv), __fmul_rn(x[i + 1], inv));
+    uint32_t c;
+    if constexpr (FMT == PXB_MX_E2M1) {
+      c = __nv_cvt_float2_to_fp4x2(y, __NV_E2M1, cudaRoundNearest);
+      if (keep) {
+        if (x[i] != 0.0f && (c & 0x07u) == 0) c |= 0x01u;
+        if (x[i + 1] != 0.0f && (c & 0x70u) == 0) c |= 0x10u;
+      }
+      out |= static_cast<uint64_t>(c & 0xffu) << (4 * i);
+    } else {
+      c = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, FMT == PXB_MX_E4M3 ? __NV_E4M3 : __NV_E5M2);
+      if (keep) {
+        if (x[i] != 0.0f && (c & 0x007fu) == 0) c |= 0x0001u;
+        if (x[i + 1] != 0.0f && (c & 0x7f00u) == 0) c |= 0x0100u;
+      }
+      out |= static_cast<uint64_t>(c & 0xffffu) << (8 * i);
+    }
+  }
+  return out;
+}
+
+// Two codes (the low 16 bits, or 8 for e2m1) -> their values before the scale.
+template <int FMT>
+__device__ __forceinline__ float2 mx_decode2(uint32_t c) {
+  __half2_raw h;
+  if constexpr (FMT == PXB_MX_E2M1) h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(c), __NV_E2M1);
+  else h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c), FMT == PXB_MX_E4M3 ? __NV_E4M3 : __NV_E5M2);
+  return __half22float2(static_cast<__half2>(h));
+}
+
+// Eight codes -> eight values before the scale.
+template <int FMT>
+__device__ __forceinline__ void mx_decode8(uint64_t codes, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint32_t half = i < (FMT == PXB_MX_E2M1 ? 8 : 4) ? static_cast<uint32_t>(codes)
+                                                            : static_cast<uint32_t>(codes >> 32);
+    const uint32_t c = FMT == PXB_MX_E2M1 ? (half >> (4 * i)) & 0xffu : (half >> (8 * (i & 3))) & 0xffffu;
+    const float2 d = mx_decode2<FMT>(c);
+    v[i] = d.x;
+    v[i + 1] = d.y;
+  }
+}
+
+// The eight codes of a lane's samples (an octet of a row: 8 bytes, or 4).
+template <int FMT>
+__device__ __forceinline__ uint64_t mx_load8(const uint8_t *__restrict__ codes, int64_t octet) {
+  if constexpr (FMT == PXB_MX_E2M1) return __ldg(reinterpret_cast<const uint32_t *>(codes) + octet);
+  else return __ldg(reinterpret_cast<const unsigned long long *>(codes) + octet);
+}
+template <int FMT>
+__device__ __forceinline__ void mx_store8(uint8_t *__restrict__ codes, int64_t octet, uint64_t v) {
+  if constexpr (FMT == PXB_MX_E2M1) reinterpret_cast<uint32_t *>(codes)[octet] = static_cast<uint32_t>(v);
+  else reinterpret_cast<unsigned long long *>(codes)[octet] = v;
+}
+
+// The largest magnitude's bits of a lane's eight values, as an unsigned order
+// in which infinities and NaN come last.
+__device__ __forceinline__ uint32_t mx_amax8(const float (&x)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  return m;
+}
+
+__host__ inline bool mx_format_ok(int fmt) { return fmt >= PXB_MX_E4M3 && fmt <= PXB_MX_E2M1; }
+
+}  // namespace pxb

@@ -13,6 +13,7 @@ A bucket is a dict of device columns named like the reference's SOA tags:
 from __future__ import annotations
 
 import ctypes
+import threading
 from collections.abc import Mapping, Sequence
 
 import torch
@@ -30,16 +31,16 @@ _DTYPES = {
 }
 
 
-_bound_device: list[int] = [-1]
+_bound = threading.local()  # the runtime's current device is one per host thread
 
 
 def _stream() -> ctypes.c_void_p:
     """The current torch stream, after binding the library's runtime to the
     current torch device (libpxb links its own CUDA runtime)."""
     dev = torch.cuda.current_device()
-    if dev != _bound_device[0]:
+    if dev != getattr(_bound, "device", -1):
         call("pxb_set_device", ctypes.c_int32(dev))
-        _bound_device[0] = dev
+        _bound.device = dev
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 

@@ -1718,12 +1718,14 @@ def gather_arena(conns, static: NetworkStatic, out: dict | None = None, group=No
 
 def make_step(net: type[Network], static: NetworkStatic, *, batch_size: int | None = None, layout: str = "auto",
               fuse_prune: str | bool = "auto", growth: str = "auto", device: torch.device | str = "cuda",
-              fuse_train: bool = True) -> StepFn:
+              fuse_train: bool = True, activation_checkpoint: str | None = None) -> StepFn:
     """Build the step for `net` on `static` (src/plastax/step.py:76-237).
 
     Raises ValueError for an unknown knob, as the reference does.
     `fuse_train=False` keeps a PIPELINE net's forward, loss, backward and
     update as separate passes where the fused training step would apply.
+    `activation_checkpoint` ("e4m3" or "e5m2", batched steps only) keeps the
+    activations that the backward pass and the update read in 8-bit blocks.
     """
     if layout not in ("auto", "edges", "csr", "triton", "xla"):
         raise ValueError(f"make_step: unknown layout {layout!r}")
@@ -1742,7 +1744,9 @@ def make_step(net: type[Network], static: NetworkStatic, *, batch_size: int | No
                              "MeanFloatFirstRest())")
         from plastax_b200.batched import BatchedStepFn
 
-        return BatchedStepFn(net, static, batch_size, torch.device(device))
+        return BatchedStepFn(net, static, batch_size, torch.device(device), activation_checkpoint)
+    if activation_checkpoint is not None:
+        raise ValueError("make_step: activation_checkpoint is for a batched step (batch_size)")
     return StepFn(net, static, torch.device(device), fuse_prune=fuse_prune is not False, fuse_train=fuse_train)
 
 

@@ -1,5 +1,7 @@
 // Edge products over microscaled rows: the gradient of every connection from
 // checkpointed activations, and the forward of a frozen arena.
+#include <cooperative_groups.h>
+
 #include "mx.cuh"
 #include "optim.cuh"
 
@@ -8,75 +10,206 @@ namespace pxb {
 // ---------------------------------------------------------------------------
 // stat[s] = (sum_b g[to, b] * a[from, b]) / B
 // ---------------------------------------------------------------------------
-// A warp owns 32 slots; eight lanes share a slot, four samples each, so one
-// load instruction covers a 32-sample slice of four slots. A lane keeps the
-// partial sums of its group's eight slots over every slice; halving them
-// across the group's lanes at the end (4 + 2 + 1 exchanges) leaves lane l
-// with slot l's sum.
-template <int FMT, bool VEC>
-__global__ void __launch_bounds__(256) mx_edge_grad_kernel(
-    int64_t cap, const int32_t *__restrict__ from, const int32_t *__restrict__ to, const uint8_t *__restrict__ dead,
-    const float *__restrict__ g, const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int32_t batch,
-    uint32_t n, float *__restrict__ dw, float *__restrict__ weight, OptParams op, float *m_col, float *v_col,
-    float *t_col) {
-  const int lane = threadIdx.x & 31, sub = lane & 7;
-  const int32_t nb = (batch + kMxBlock - 1) / kMxBlock;
-  const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
-  for (int64_t base = ((blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5) * 32; base < cap;
-       base += warps * 32) {
-    const int64_t s = base + lane;
-    int32_t f = -1, t = -1;
-    if (s < cap && !dead[s]) {
-      f = from[s];
-      t = to[s];
-      if (static_cast<uint32_t>(f) >= n || static_cast<uint32_t>(t) >= n) f = t = -1;
-    }
-    float p[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (__any_sync(0xffffffffu, t >= 0)) {
-      for (int32_t k = 0; k < nb; ++k) {
-        const int32_t b = k * kMxBlock + sub * 4;
+struct EdgeGrad {
+  int64_t cap;
+  const int32_t *__restrict__ from, *__restrict__ to;
+  const uint8_t *__restrict__ dead;
+  const float *__restrict__ g;
+  const uint8_t *__restrict__ codes, *__restrict__ scales;
+  int32_t batch, nb;
+  uint32_t n;
+  float *dw, *weight;
+  OptParams op;
+  float *m, *v, *t;
+};
+
+// A slot as it was read (three loads in flight together), and whether it
+// takes a gradient.
+struct Slot {
+  int32_t f, t;
+  uint8_t dead;
+  __device__ __forceinline__ bool live(uint32_t n) const {
+    return !dead && static_cast<uint32_t>(f) < n && static_cast<uint32_t>(t) < n;
+  }
+};
+
+__device__ __forceinline__ Slot load_slot(const EdgeGrad &k, int64_t s) {
+  Slot r{0, 0, 1};
+  if (s < k.cap) r = Slot{__ldg(k.from + s), __ldg(k.to + s), __ldg(k.dead + s)};
+  return r;
+}
+
+// Offsets into the gradient rows and the codes: 32 bits where the rows end
+// below 4 GiB (one add a load, from a uniform base), else 64.
+template <bool WIDE>
+struct Offset {
+  using type = uint32_t;
+};
+template <>
+struct Offset<true> {
+  using type = uint64_t;
+};
+
+// Four gradients from byte offset `at`, whose first sample is b: 0 past the
+// batch (FULL: the whole slice lies below it).
+template <bool VEC, bool FULL, typename O>
+__device__ __forceinline__ float4 load_grad(const float *__restrict__ g, O at, int32_t batch, int32_t b) {
+  const float *p = reinterpret_cast<const float *>(reinterpret_cast<const char *>(g) + at);
+  if (VEC && FULL) return __ldg(reinterpret_cast<const float4 *>(p));
+  if (!VEC && FULL) return make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (VEC) {
+    if (b < batch) v = __ldg(reinterpret_cast<const float4 *>(p));
+    return v;
+  }
+  if (b < batch) v.x = __ldg(p);
+  if (b + 1 < batch) v.y = __ldg(p + 1);
+  if (b + 2 < batch) v.z = __ldg(p + 2);
+  if (b + 3 < batch) v.w = __ldg(p + 3);
+  return v;
+}
+
+// A lane's four activations of a slice of source row f, as two pairs.
+template <int FMT, typename O>
+__device__ __forceinline__ void load_acts(const EdgeGrad &k, int32_t f, int32_t slice, int sub, float2 (&a)[2]) {
+  const O blk = static_cast<O>(f) * static_cast<O>(k.nb) + static_cast<O>(slice);
+  const uint32_t c = __ldg(reinterpret_cast<const uint32_t *>(k.codes + blk * 32) + sub);
+  const float sc = mx_scale_value(__ldg(k.scales + blk));
+  const float2 lo = mx_decode2<FMT>(c & 0xffffu), hi = mx_decode2<FMT>(c >> 16);
+  a[0] = make_float2(__fmul_rn(lo.x, sc), __fmul_rn(lo.y, sc));
+  a[1] = make_float2(__fmul_rn(hi.x, sc), __fmul_rn(hi.y, sc));
+}
+
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long &>(d))
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
+        "l"(reinterpret_cast<unsigned long long &>(c)));
+  return d;
+}
+
+// One slice of slot_sums: the group's eight slots' products into p. UNIFORM:
+// their source is `f` for the whole group.
+template <int FMT, bool VEC, bool FULL, bool UNIFORM, int DEPTH, typename O>
+__device__ __forceinline__ void slice_sums(const EdgeGrad &k, int32_t f, O row, int32_t slice, float2 (&p)[8]) {
+  const int sub = threadIdx.x & 7;
+  const int32_t b = slice * kMxBlock + sub * 4;
+  float2 a[2];
+  int32_t cur = UNIFORM ? f : __shfl_sync(0xffffffffu, f, 0, 8);
+  load_acts<FMT, O>(k, cur, slice, sub, a);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int32_t fj = __shfl_sync(0xffffffffu, f, j, 8), tj = __shfl_sync(0xffffffffu, t, j, 8);
-          if (tj < 0) continue;
-          const float *gr = g + static_cast<int64_t>(tj) * batch + b;
-          float4 gv = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (VEC) {
-            if (b < batch) gv = __ldg(reinterpret_cast<const float4 *>(gr));
-          } else {
-            if (b < batch) gv.x = __ldg(gr);
-            if (b + 1 < batch) gv.y = __ldg(gr + 1);
-            if (b + 2 < batch) gv.z = __ldg(gr + 2);
-            if (b + 3 < batch) gv.w = __ldg(gr + 3);
-          }
-          const int64_t blk = static_cast<int64_t>(fj) * nb + k;
-          const uint32_t c = __ldg(reinterpret_cast<const uint32_t *>(codes) + blk * 8 + sub);
-          const float2 lo = mx_decode2<FMT>(c & 0xffffu), hi = mx_decode2<FMT>(c >> 16);
-          const float dot = gv.x * lo.x + gv.y * lo.y + gv.z * hi.x + gv.w * hi.y;
-          p[j] = fmaf(dot, mx_scale_value(__ldg(scales + blk)), p[j]);
+  for (int j0 = 0; j0 < 8; j0 += DEPTH) {
+    float4 gv[DEPTH];
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j)
+      gv[j] = load_grad<VEC, FULL, O>(k.g, __shfl_sync(0xffffffffu, row, j0 + j, 8) + static_cast<O>(b) * 4, k.batch, b);
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) {
+      if (!UNIFORM) {
+        const int32_t fj = __shfl_sync(0xffffffffu, f, j0 + j, 8);
+        if (fj != cur) {
+          cur = fj;
+          load_acts<FMT, O>(k, fj, slice, sub, a);
         }
       }
-#pragma unroll
-      for (int half = 4; half > 0; half >>= 1) {
-        const bool upper = (lane & half) != 0;
-#pragma unroll
-        for (int i = 0; i < half; ++i) {
-          const float send = upper ? p[i] : p[i + half], keep = upper ? p[i + half] : p[i];
-          p[i] = keep + __shfl_xor_sync(0xffffffffu, send, half);
-        }
-      }
-    }
-    if (s < cap) {
-      const float stat = __fdiv_rn(p[0], static_cast<float>(batch));
-      if (dw != nullptr) {
-        dw[s] = t >= 0 ? stat : 0.0f;
-      } else if (t >= 0) {
-        float w = weight[s];
-        opt_step(op, stat, w, m_col, v_col, t_col, s);
-        weight[s] = w;
-      }
+      p[j0 + j] = ffma2(make_float2(gv[j].x, gv[j].y), a[0], p[j0 + j]);
+      p[j0 + j] = ffma2(make_float2(gv[j].z, gv[j].w), a[1], p[j0 + j]);
     }
   }
+}
+
+// sum_b g[to, b] * a[from, b] over the slices first, first + step, ... of the
+// warp's 32 slots; lane l returns slot l's. Eight lanes share a slot, four
+// samples each, so one load instruction covers a 32-sample slice of four
+// slots. A lane keeps the partial sums of its group's eight slots over every
+// slice; halving them across the group's lanes at the end (4 + 2 + 1
+// exchanges) leaves each lane its own slot's sum. The arena is source-major but
+// for regrown slots: where each group's slots share a source, its codes are
+// read and widened once a slice, else once a run.
+template <int FMT, bool VEC, bool WIDE, int DEPTH>
+__device__ __forceinline__ float slot_sums(const EdgeGrad &k, const Slot &slot, int first, int step) {
+  using O = typename Offset<WIDE>::type;
+  const bool mine = slot.live(k.n);
+  const unsigned live = __ballot_sync(0xffffffffu, mine);
+  if (live == 0) return 0.0f;
+  const int lane = threadIdx.x & 31;
+  // a slot without a gradient stands at its group's first source and at row 0: its sum is not read
+  const int lead = __ffs(live >> (lane & 24) & 0xffu) - 1;
+  const int32_t first_f = __shfl_sync(0xffffffffu, mine ? slot.f : 0, lead < 0 ? 0 : lead, 8);
+  const int32_t f = mine ? slot.f : first_f;
+  const bool uniform = __all_sync(0xffffffffu, f == first_f);
+  const O row = static_cast<O>(mine ? slot.t : 0) * static_cast<O>(k.batch) * 4;
+  float2 p[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p[j] = make_float2(0.0f, 0.0f);
+  for (int32_t slice = first; slice < k.nb; slice += step) {
+    const bool full = (slice + 1) * kMxBlock <= k.batch;
+    if (full && uniform) slice_sums<FMT, VEC, true, true, DEPTH, O>(k, f, row, slice, p);
+    else if (full) slice_sums<FMT, VEC, true, false, DEPTH, O>(k, f, row, slice, p);
+    else slice_sums<FMT, VEC, false, false, DEPTH, O>(k, f, row, slice, p);
+  }
+  float q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q[j] = p[j].x + p[j].y;
+#pragma unroll
+  for (int half = 4; half > 0; half >>= 1) {
+    const bool upper = (lane & half) != 0;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float send = upper ? q[i] : q[i + half], keep = upper ? q[i + half] : q[i];
+      q[i] = keep + __shfl_xor_sync(0xffffffffu, send, half);
+    }
+  }
+  return q[0];
+}
+
+__device__ __forceinline__ void finish_slot(const EdgeGrad &k, int64_t s, bool live, float sum) {
+  const float stat = __fdiv_rn(sum, static_cast<float>(k.batch));
+  if (k.dw != nullptr) {
+    k.dw[s] = live ? stat : 0.0f;
+  } else if (live) {
+    float w = k.weight[s];
+    opt_step(k.op, stat, w, k.m, k.v, k.t, s);
+    k.weight[s] = w;
+  }
+}
+
+// Every warp takes 32 slots at a time over the whole batch. What costs is the
+// gradient rows, 128 bytes a slot and slice. Rows that an L1 can hold in part
+// gain from it, and more warps an SM would only push them out; larger ones come
+// from L2 whatever the L1 does, and want the loads of a fourth block an SM
+// (MIN_BLOCKS).
+template <int FMT, bool VEC, bool WIDE, int MIN_BLOCKS>
+__global__ void __launch_bounds__(256, MIN_BLOCKS) mx_edge_grad_kernel(EdgeGrad k) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t s = blockIdx.x * int64_t(256) + threadIdx.x; s - (threadIdx.x & 31) < k.cap; s += stride) {
+    const Slot slot = load_slot(k, s);
+    const float sum = slot_sums<FMT, VEC, WIDE, 8>(k, slot, 0, 1);
+    if (s < k.cap) finish_slot(k, s, slot.live(k.n), sum);
+  }
+}
+
+// Few slots and a long batch: the CTAs of a cluster share 256 slots, CTA r
+// taking the slices r, r + ranks, ...; the partial sums join through the
+// cluster's shared memory in rank order.
+template <int FMT, bool VEC, bool WIDE>
+__global__ void __launch_bounds__(256) mx_edge_grad_split_kernel(EdgeGrad k) {
+  namespace cg = cooperative_groups;
+  __shared__ float part[256];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int64_t base = blockIdx.x / ranks * int64_t(256);
+  const Slot slot = load_slot(k, base + threadIdx.x);
+  part[threadIdx.x] = slot_sums<FMT, VEC, WIDE, 8>(k, slot, rank, ranks);
+  cluster.sync();
+  const int at = static_cast<int>(threadIdx.x), share = 256 / ranks;
+  if (at / share == rank && base + at < k.cap) {
+    float sum = 0.0f;
+    for (int r = 0; r < ranks; ++r) sum += cluster.map_shared_rank(part, r)[at];
+    finish_slot(k, base + at, slot.live(k.n), sum);
+  }
+  cluster.sync();  // the peers have read this CTA's sums
 }
 
 // ---------------------------------------------------------------------------
@@ -138,103 +271,249 @@ struct Rows {
   const uint8_t *__restrict__ codes;
   const uint8_t *__restrict__ scales;
   int32_t batch, nb;
+
+  // samples in the 16 bytes that a lane loads at once, and the lanes a row takes at most
+  static constexpr int kPiece = XF == PXB_MX_F32 ? 4 : XF == PXB_MX_E2M1 ? 32 : 16;
+  static constexpr int kMaxLanes = XF == PXB_MX_F32 ? 32 : 256 / kPiece;
 };
 
-// A warp owns one destination and a chunk of 256 samples. A lane holds eight
-// consecutive samples; where a row has fewer than 32 octets, 32 / LANES edges
-// run side by side and their sums join at the end by shuffles.
-template <int XF, int LANES, bool VEC>
-__global__ void __launch_bounds__(256) mx_product_kernel(Conns c, uint32_t num_src, Rows<XF> r, int act_kind, Out out,
-                                                         int32_t chunks) {
-  constexpr int kGroups = 32 / LANES;
-  const int lane = threadIdx.x & 31, sub = lane % LANES, grp = lane / LANES;
-  const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
-  const int64_t total = static_cast<int64_t>(c.num_dst) * chunks;
-  for (int64_t item = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5; item < total;
-       item += warps) {
-    const int32_t i = static_cast<int32_t>(item / chunks);
-    const int32_t b = static_cast<int32_t>(item - static_cast<int64_t>(i) * chunks) * 256 + sub * 8;
-    const int64_t e0 = max(int64_t(0), c.offsets[i]), e1 = min(c.num_edges, c.offsets[i + 1]);
-    const int64_t blk0 = c.fmt == PXB_MX_F32 ? 0 : max(int64_t(0), c.block_offsets[i]);
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int64_t e = e0; e < e1; e += 32) {
-      int32_t s = -1;
-      float w = 0.0f;
-      if (e + lane < e1) {
-        s = __ldg(c.src + e + lane);
-        if (static_cast<uint32_t>(s) >= num_src) s = -1;
-        w = conn_weight(c, e + lane, blk0 + ((e - e0) >> 5), lane);
-      }
-      const int cnt = static_cast<int>(min(int64_t(32), e1 - e));
-      for (int j = 0; j < cnt; j += kGroups) {
-        const int32_t sj = __shfl_sync(0xffffffffu, s, j + grp);
-        const float wj = __shfl_sync(0xffffffffu, w, j + grp);
-        if (sj < 0 || b >= r.batch) continue;
-        float v[8];
-        if constexpr (XF == PXB_MX_F32) {
-          const float *xr = r.x + static_cast<int64_t>(sj) * r.batch + b;
-          if (VEC && b + 8 <= r.batch) {
-            const float4 lo = __ldg(reinterpret_cast<const float4 *>(xr));
-            const float4 hi = __ldg(reinterpret_cast<const float4 *>(xr) + 1);
-            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-          } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = b + q < r.batch ? __ldg(xr + q) : 0.0f;
-          }
-#pragma unroll
-          for (int q = 0; q < 8; ++q) acc[q] = fmaf(wj, v[q], acc[q]);
-        } else {
-          const int64_t row = static_cast<int64_t>(sj) * r.nb;
-          mx_decode8<XF>(mx_load8<XF>(r.codes, row * 4 + (b >> 3)), v);
-          const float ws = __fmul_rn(wj, mx_scale_value(__ldg(r.scales + row + (b >> 5))));
-#pragma unroll
-          for (int q = 0; q < 8; ++q) acc[q] = fmaf(ws, v[q], acc[q]);
-        }
-      }
-    }
-#pragma unroll
-    for (int off = LANES; off < 32; off <<= 1)
-#pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] += __shfl_xor_sync(0xffffffffu, acc[q], off);
-    const int32_t u = c.units[i];
-    const bool on = grp == 0 && b < r.nb * kMxBlock && static_cast<uint32_t>(u) < out.rows;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) acc[q] = b + q < r.batch ? act_fn(act_kind, acc[q]) : 0.0f;
-    if (out.fmt == PXB_MX_F32) {
-      float *o = out.x + static_cast<int64_t>(u) * r.batch + b;
-      if (on && VEC && b + 8 <= r.batch) {
-        reinterpret_cast<float4 *>(o)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        reinterpret_cast<float4 *>(o)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      } else if (on) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (b + q < r.batch) o[q] = acc[q];
-      }
+// One loaded piece of a source row and the factor of its values.
+struct Piece {
+  uint4 v;
+  float w;
+};
+
+template <int XF, bool VEC>
+__device__ __forceinline__ Piece load_piece(const Rows<XF> &r, int32_t src, float w, int32_t piece, bool on) {
+  Piece p{make_uint4(0, 0, 0, 0), 0.0f};
+  if (!on || src < 0) return p;
+  if constexpr (XF == PXB_MX_F32) {
+    const int32_t b = piece * 4;
+    const float *x = r.x + static_cast<int64_t>(src) * r.batch + b;
+    p.w = w;
+    if (VEC) {
+      p.v = __ldg(reinterpret_cast<const uint4 *>(x));
     } else {
-      const int64_t o = static_cast<int64_t>(u) * r.nb * 4 + (b >> 3);
-      if (out.fmt == PXB_MX_E4M3) store_codes<PXB_MX_E4M3>(acc, on, o, out.codes, out.scales);
-      else if (out.fmt == PXB_MX_E5M2) store_codes<PXB_MX_E5M2>(acc, on, o, out.codes, out.scales);
-      else store_codes<PXB_MX_E2M1>(acc, on, o, out.codes, out.scales);
+      const uint32_t *u = reinterpret_cast<const uint32_t *>(x);
+      p.v.x = __ldg(u);
+      if (b + 1 < r.batch) p.v.y = __ldg(u + 1);
+      if (b + 2 < r.batch) p.v.z = __ldg(u + 2);
+      if (b + 3 < r.batch) p.v.w = __ldg(u + 3);
     }
+  } else {
+    constexpr int kPerBlock = kMxBlock / Rows<XF>::kPiece;
+    const int64_t row = static_cast<int64_t>(src) * r.nb;
+    p.v = __ldg(reinterpret_cast<const uint4 *>(r.codes) + row * kPerBlock + piece);
+    p.w = __fmul_rn(w, mx_scale_value(__ldg(r.scales + row + piece / kPerBlock)));
+  }
+  return p;
+}
+
+// acc += w * values, two at a time.
+template <int XF>
+__device__ __forceinline__ void add_piece(const Piece &p, float2 (&acc)[Rows<XF>::kPiece / 2]) {
+  const uint32_t v[4] = {p.v.x, p.v.y, p.v.z, p.v.w};
+  const float2 w = make_float2(p.w, p.w);
+  if constexpr (XF == PXB_MX_F32) {
+    acc[0] = ffma2(w, make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), acc[0]);
+    acc[1] = ffma2(w, make_float2(__uint_as_float(v[2]), __uint_as_float(v[3])), acc[1]);
+  } else if constexpr (XF == PXB_MX_E2M1) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = ffma2(w, mx_decode2<XF>((v[i >> 2] >> (8 * (i & 3))) & 0xffu), acc[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = ffma2(w, mx_decode2<XF>((v[i >> 1] >> (16 * (i & 1))) & 0xffffu), acc[i]);
   }
 }
 
-template <int XF>
+// The edges of a destination are cut into blocks of 32 (the weights' blocks).
+// A warp takes a block: lane j holds edge j's source and weight. A source row
+// is LANES pieces of 16 bytes (a whole block of 32 samples in e2m1, 16 samples
+// in 8 bits, 4 in float32), so 32 / LANES edges are read side by side, each
+// load instruction full, up to four in flight a lane. `wpd` warps of a block
+// and, where destinations are few and long, the CTAs of a cluster share a
+// destination's blocks; their sums join in shared memory (a peer CTA's through
+// the cluster) in a fixed order, and one octet a thread then takes the
+// activation and leaves as float32 or as codes.
+template <int XF, int LANES, bool VEC>
+__global__ void __launch_bounds__(256) mx_product_kernel(Conns c, uint32_t num_src, Rows<XF> r, int act_kind, Out out,
+                                                         int32_t chunks, int wpd) {
+  constexpr int A = Rows<XF>::kPiece, kGroups = 32 / LANES, kChunk = LANES * A;
+  constexpr int kOctets = (kChunk < kMxBlock ? kMxBlock : kChunk) / 8;  // an item's octets: whole blocks
+  constexpr int kDepth = LANES < 4 ? LANES : 4;
+  __shared__ float part[8][kChunk];
+  namespace cg = cooperative_groups;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES, grp = lane / LANES;
+  const int team = warp / wpd, member = warp % wpd, per_cta = 8 / wpd;
+  const int32_t pieces = XF == PXB_MX_F32 ? (r.batch + 3) / 4 : r.nb * (kMxBlock / A);
+  const int64_t total = static_cast<int64_t>(c.num_dst) * chunks, tiles = (total + per_cta - 1) / per_cta;
+  for (int64_t tile = blockIdx.x / ranks; tile < tiles; tile += gridDim.x / ranks) {
+    const int64_t item = tile * per_cta + team;
+    float2 acc[A / 2];
+#pragma unroll
+    for (int q = 0; q < A / 2; ++q) acc[q] = make_float2(0.0f, 0.0f);
+    if (item < total) {
+      const int32_t i = static_cast<int32_t>(item / chunks);
+      const int32_t piece = static_cast<int32_t>(item - static_cast<int64_t>(i) * chunks) * LANES + sub;
+      const bool on = piece < pieces;
+      const int64_t e0 = max(int64_t(0), __ldg(c.offsets + i)), e1 = min(c.num_edges, __ldg(c.offsets + i + 1));
+      const int64_t blk0 = c.fmt == PXB_MX_F32 ? 0 : max(int64_t(0), __ldg(c.block_offsets + i));
+      for (int64_t k = member + rank * wpd; e0 + k * 32 < e1; k += wpd * ranks) {
+        const int64_t e = e0 + k * 32 + lane;
+        int32_t s = -1;
+        float w = 0.0f;
+        if (e < e1) {
+          s = __ldg(c.src + e);
+          if (static_cast<uint32_t>(s) >= num_src) s = -1;
+          w = conn_weight(c, e, blk0 + k, lane);
+        }
+        const int cnt = static_cast<int>(min(int64_t(32), e1 - e0 - k * 32));
+#pragma unroll 1
+        for (int j = 0; j < cnt; j += kGroups * kDepth) {
+          Piece p[kDepth];
+#pragma unroll
+          for (int d = 0; d < kDepth; ++d) {
+            const int at = j + d * kGroups + grp;
+            p[d] = load_piece<XF, VEC>(r, __shfl_sync(0xffffffffu, s, at), __shfl_sync(0xffffffffu, w, at), piece, on);
+          }
+#pragma unroll
+          for (int d = 0; d < kDepth; ++d) add_piece<XF>(p[d], acc);
+        }
+      }
+    }
+    // the edges read side by side join: halves of the samples go to the other side until one is left
+    float f[A];
+#pragma unroll
+    for (int q = 0; q < A / 2; ++q) f[2 * q] = acc[q].x, f[2 * q + 1] = acc[q].y;
+    int base = sub * A;
+    constexpr int kHeld = A > kGroups ? A / kGroups : 1;
+#pragma unroll
+    for (int off = 16, n = A; off >= LANES; off >>= 1) {
+      if (n > 1) {
+        n >>= 1;
+        const bool upper = (lane & off) != 0;
+#pragma unroll
+        for (int q = 0; q < n; ++q) {
+          const float send = upper ? f[q] : f[q + n], keep = upper ? f[q + n] : f[q];
+          f[q] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+        }
+        base += upper ? n : 0;
+      } else {
+        f[0] += __shfl_xor_sync(0xffffffffu, f[0], off);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kHeld; ++q) part[warp][base + q] = f[q];
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+    if (rank == 0) {
+      // every warp steps through whole rounds, so that a block's four lanes meet in the shuffles
+      for (int t = threadIdx.x; t < ((per_cta * kOctets + 31) & ~31); t += 256) {
+        const int j = t / kOctets, o = (t - j * kOctets) * 8;
+        const int64_t it = tile * per_cta + j;
+        const bool live = j < per_cta && it < total;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        int32_t u = -1, b = 0;
+        if (live) {
+          const int32_t i = static_cast<int32_t>(it / chunks);
+          u = __ldg(c.units + i);
+          b = static_cast<int32_t>(it - static_cast<int64_t>(i) * chunks) * kChunk + o;
+          for (int k = 0; k < ranks; ++k) {
+            const float *q = ranks > 1 ? cluster.map_shared_rank(&part[0][0], k) : &part[0][0];
+            for (int m = 0; m < wpd; ++m)
+#pragma unroll
+              for (int z = 0; z < 8; ++z)
+                if (o + z < kChunk) v[z] += q[(j * wpd + m) * kChunk + o + z];
+          }
+#pragma unroll
+          for (int z = 0; z < 8; ++z) v[z] = b + z < r.batch ? act_fn(act_kind, v[z]) : 0.0f;
+        }
+        const bool on = live && b < r.nb * kMxBlock && static_cast<uint32_t>(u) < out.rows;
+        if (out.fmt == PXB_MX_F32) {
+          float *dst = out.x + static_cast<int64_t>(u) * r.batch + b;
+          if (on && VEC && b + 8 <= r.batch) {
+            reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else if (on) {
+#pragma unroll
+            for (int z = 0; z < 8; ++z)
+              if (b + z < r.batch) dst[z] = v[z];
+          }
+        } else {
+          const int64_t at = static_cast<int64_t>(u) * r.nb * 4 + (b >> 3);
+          if (out.fmt == PXB_MX_E4M3) store_codes<PXB_MX_E4M3>(v, on, at, out.codes, out.scales);
+          else if (out.fmt == PXB_MX_E5M2) store_codes<PXB_MX_E5M2>(v, on, at, out.codes, out.scales);
+          else store_codes<PXB_MX_E2M1>(v, on, at, out.codes, out.scales);
+        }
+      }
+    }
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+  }
+}
+
+template <int XF, int LANES, bool VEC>
+static int launch_product_as(const Conns &c, int32_t num_src, const Rows<XF> &r, int act, const Out &out, int32_t chunks,
+                             cudaStream_t st) {
+  const int64_t items = static_cast<int64_t>(c.num_dst) * chunks, mean = c.num_edges / c.num_dst;
+  const int64_t warps = static_cast<int64_t>(sm_count()) * 32;
+  int wpd = 1, ranks = 1;
+  while (wpd < 8 && items * wpd < warps && mean > 32 * wpd) wpd *= 2;
+  if (wpd == 8)
+    while (ranks < 8 && items * 8 * ranks < warps && mean > 32 * 8 * ranks) ranks *= 2;
+  const int64_t tiles = (items * wpd + 7) / 8, most = static_cast<int64_t>(sm_count()) * 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((tiles < most ? tiles : most) * ranks));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  PXB_CUDA(cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, LANES, VEC>, c, static_cast<uint32_t>(num_src), r, act, out,
+                              chunks, wpd));
+  return PXB_OK;
+}
+
+template <int XF, int LANES>
 static int launch_product(const Conns &c, int32_t num_src, const Rows<XF> &r, int act, const Out &out, bool vec,
                           cudaStream_t st) {
-  const int32_t octets = r.nb * 4, chunks = (octets + 31) / 32;
-  const int grid = grid_for(static_cast<int64_t>(c.num_dst) * chunks, 8, 8);
-#define PXB_MXP(L)                                                                                         \
-  do {                                                                                                     \
-    if (vec) mx_product_kernel<XF, L, true><<<grid, 256, 0, st>>>(c, num_src, r, act, out, chunks);         \
-    else mx_product_kernel<XF, L, false><<<grid, 256, 0, st>>>(c, num_src, r, act, out, chunks);            \
-  } while (0)
-  if (octets <= 4) PXB_MXP(4);
-  else if (octets <= 8) PXB_MXP(8);
-  else if (octets <= 16) PXB_MXP(16);
-  else PXB_MXP(32);
-#undef PXB_MXP
-  PXB_LAUNCHED("mx_product_kernel");
+  const int32_t pieces = XF == PXB_MX_F32 ? (r.batch + 3) / 4 : r.nb * (kMxBlock / Rows<XF>::kPiece);
+  if constexpr (LANES < Rows<XF>::kMaxLanes) {
+    if (pieces > LANES) return launch_product<XF, LANES * 2>(c, num_src, r, act, out, vec, st);
+  }
+  const int32_t chunks = (pieces + LANES - 1) / LANES;
+  if (vec) return launch_product_as<XF, LANES, true>(c, num_src, r, act, out, chunks, st);
+  return launch_product_as<XF, LANES, false>(c, num_src, r, act, out, chunks, st);
+}
+
+template <int FMT, bool VEC, bool WIDE>
+static int launch_edge_grad(const EdgeGrad &k, cudaStream_t st) {
+  const int64_t blocks = (k.cap + 255) / 256;
+  int ranks = 1;
+  while (ranks < 8 && ranks * 2 <= k.nb && blocks * ranks <= sm_count()) ranks *= 2;
+  if (ranks > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks * ranks));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ranks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    PXB_CUDA(cudaLaunchKernelEx(&cfg, mx_edge_grad_split_kernel<FMT, VEC, WIDE>, k));
+    return PXB_OK;
+  }
+  const int grid = grid_for((k.cap + 31) / 32, 8, 8);
+  if (k.n <= 4096) mx_edge_grad_kernel<FMT, VEC, WIDE, 3><<<grid, 256, 0, st>>>(k);
+  else mx_edge_grad_kernel<FMT, VEC, WIDE, 4><<<grid, 256, 0, st>>>(k);
+  PXB_LAUNCHED("mx_edge_grad_kernel");
   return PXB_OK;
 }
 
@@ -261,23 +540,18 @@ extern "C" int pxb_mx_edge_grad(int64_t cap, const int32_t *from_id, const int32
     PXB_REQUIRE(opt->kind != PXB_OPT_ADAM || (opt_m && opt_t), "pxb_mx_edge_grad: adam needs opt/m and opt/t");
     op = OptParams{opt->kind, opt->lr, opt->b1, opt->b2, opt->eps, opt->weight_decay, nullptr};
   }
-  const int grid = grid_for((cap + 31) / 32, 8, 8);
-  cudaStream_t st = as_stream(stream);
   const bool vec = aligned16(g) && batch % 4 == 0;
-  const uint32_t n = static_cast<uint32_t>(num_units);
-#define PXB_EG(F, V)                                                                                               \
-  mx_edge_grad_kernel<F, V><<<grid, 256, 0, st>>>(cap, from_id, to_id, dead, g, codes, scales, batch, n, dw, weight, \
-                                                  op, opt_m, opt_v, opt_t)
-  if (fmt == PXB_MX_E4M3) {
-    if (vec) PXB_EG(PXB_MX_E4M3, true);
-    else PXB_EG(PXB_MX_E4M3, false);
-  } else {
-    if (vec) PXB_EG(PXB_MX_E5M2, true);
-    else PXB_EG(PXB_MX_E5M2, false);
-  }
+  const EdgeGrad k{cap, from_id, to_id, dead, g, codes, scales, batch,
+                   static_cast<int32_t>(mx_blocks(batch)), static_cast<uint32_t>(num_units), dw, weight, op, opt_m,
+                   opt_v, opt_t};
+  cudaStream_t st = as_stream(stream);
+  const bool wide = !vec || static_cast<int64_t>(num_units) * batch * 4 >= (int64_t(1) << 32);
+#define PXB_EG(F) \
+  return !vec ? launch_edge_grad<F, false, true>(k, st) \
+              : wide ? launch_edge_grad<F, true, true>(k, st) : launch_edge_grad<F, true, false>(k, st)
+  if (fmt == PXB_MX_E4M3) PXB_EG(PXB_MX_E4M3);
+  PXB_EG(PXB_MX_E5M2);
 #undef PXB_EG
-  PXB_LAUNCHED("mx_edge_grad_kernel");
-  return PXB_OK;
 }
 
 extern "C" int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src, int32_t batch, const float *x,
@@ -310,7 +584,7 @@ extern "C" int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src, int32_
   cudaStream_t st = as_stream(stream);
   const Out o{out_fmt, static_cast<uint32_t>(num_out), out, out_codes, out_scales};
 #define PXB_MXD(XF) \
-  launch_product<XF>(c, num_src, Rows<XF>{x, x_codes, x_scales, batch, nb}, act_kind, o, vec, st)
+  launch_product<XF, kMxBlock / (XF == PXB_MX_F32 ? kMxBlock : Rows<XF>::kPiece)>(c, num_src, Rows<XF>{x, x_codes, x_scales, batch, nb}, act_kind, o, vec, st)
   if (x_fmt == PXB_MX_F32) return PXB_MXD(PXB_MX_F32);
   if (x_fmt == PXB_MX_E4M3) return PXB_MXD(PXB_MX_E4M3);
   if (x_fmt == PXB_MX_E5M2) return PXB_MXD(PXB_MX_E5M2);

@@ -98,26 +98,45 @@ __device__ __forceinline__ uint64_t mx_encode8(const float (&x)[8], uint32_t sca
   return out;
 }
 
-// Two codes (the low 16 bits, or 8 for e2m1) -> their values before the scale.
+// Four bytes of codes (4 in 8 bits, 8 in e2m1) -> pairs of values before the
+// scale. Every element is a half; the conversions are the hardware's.
 template <int FMT>
-__device__ __forceinline__ float2 mx_decode2(uint32_t c) {
-  __half2_raw h;
-  if constexpr (FMT == PXB_MX_E2M1) h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(c), __NV_E2M1);
-  else h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c), FMT == PXB_MX_E4M3 ? __NV_E4M3 : __NV_E5M2);
-  return __half22float2(static_cast<__half2>(h));
+__device__ __forceinline__ void mx_decode_word(uint32_t c, __half2 (&h)[32 / (2 * MxFormat<FMT>::bits)]) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(h);
+  if constexpr (FMT == PXB_MX_E2M1)
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(c));
+  else if constexpr (FMT == PXB_MX_E4M3)
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(r[0]), "=r"(r[1]) : "r"(c));
+  else
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e5m2x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e5m2x2 %1, b;\n\t}" : "=r"(r[0]), "=r"(r[1]) : "r"(c));
+}
+
+// The value of one code.
+template <int FMT>
+__device__ __forceinline__ float mx_decode1(uint32_t c) {
+  __half2 h[32 / (2 * MxFormat<FMT>::bits)];
+  mx_decode_word<FMT>(c, h);
+  return __low2float(h[0]);
 }
 
 // Eight codes -> eight values before the scale.
 template <int FMT>
 __device__ __forceinline__ void mx_decode8(uint64_t codes, float (&v)[8]) {
+  constexpr int kWords = FMT == PXB_MX_E2M1 ? 1 : 2, kPairs = 4 / kWords;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const uint32_t half = i < (FMT == PXB_MX_E2M1 ? 8 : 4) ? static_cast<uint32_t>(codes)
-                                                            : static_cast<uint32_t>(codes >> 32);
-    const uint32_t c = FMT == PXB_MX_E2M1 ? (half >> (4 * i)) & 0xffu : (half >> (8 * (i & 3))) & 0xffffu;
-    const float2 d = mx_decode2<FMT>(c);
-    v[i] = d.x;
-    v[i + 1] = d.y;
+  for (int w = 0; w < kWords; ++w) {
+    __half2 h[kPairs];
+    mx_decode_word<FMT>(static_cast<uint32_t>(codes >> (32 * w)), h);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const float2 d = __half22float2(h[i]);
+      v[(w * kPairs + i) * 2] = d.x;
+      v[(w * kPairs + i) * 2 + 1] = d.y;
+    }
   }
 }
 

@@ -75,7 +75,9 @@ __device__ __forceinline__ void load_acts(const EdgeGrad &k, int32_t f, int32_t 
   const O blk = static_cast<O>(f) * static_cast<O>(k.nb) + static_cast<O>(slice);
   const uint32_t c = __ldg(reinterpret_cast<const uint32_t *>(k.codes + blk * 32) + sub);
   const float sc = mx_scale_value(__ldg(k.scales + blk));
-  const float2 lo = mx_decode2<FMT>(c & 0xffffu), hi = mx_decode2<FMT>(c >> 16);
+  __half2 h[2];
+  mx_decode_word<FMT>(c, h);
+  const float2 lo = __half22float2(h[0]), hi = __half22float2(h[1]);
   a[0] = make_float2(__fmul_rn(lo.x, sc), __fmul_rn(lo.y, sc));
   a[1] = make_float2(__fmul_rn(hi.x, sc), __fmul_rn(hi.y, sc));
 }
@@ -234,10 +236,10 @@ __device__ __forceinline__ float conn_weight(const Conns &c, int64_t edge, int64
   const float s = mx_scale_value(__ldg(c.scales + blk));
   float v;
   if (c.fmt == PXB_MX_E2M1) {
-    v = mx_decode2<PXB_MX_E2M1>((__ldg(c.codes + blk * 16 + (at >> 1)) >> (4 * (at & 1))) & 0xfu).x;
+    v = mx_decode1<PXB_MX_E2M1>(__ldg(c.codes + blk * 16 + (at >> 1)) >> (4 * (at & 1)));
   } else {
     const uint32_t code = __ldg(c.codes + blk * 32 + at);
-    v = c.fmt == PXB_MX_E4M3 ? mx_decode2<PXB_MX_E4M3>(code).x : mx_decode2<PXB_MX_E5M2>(code).x;
+    v = c.fmt == PXB_MX_E4M3 ? mx_decode1<PXB_MX_E4M3>(code) : mx_decode1<PXB_MX_E5M2>(code);
   }
   return __fmul_rn(v, s);
 }
@@ -317,12 +319,15 @@ __device__ __forceinline__ void add_piece(const Piece &p, float2 (&acc)[Rows<XF>
   if constexpr (XF == PXB_MX_F32) {
     acc[0] = ffma2(w, make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), acc[0]);
     acc[1] = ffma2(w, make_float2(__uint_as_float(v[2]), __uint_as_float(v[3])), acc[1]);
-  } else if constexpr (XF == PXB_MX_E2M1) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = ffma2(w, mx_decode2<XF>((v[i >> 2] >> (8 * (i & 3))) & 0xffu), acc[i]);
   } else {
+    constexpr int kPairs = 32 / (2 * MxFormat<XF>::bits);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = ffma2(w, mx_decode2<XF>((v[i >> 1] >> (16 * (i & 1))) & 0xffffu), acc[i]);
+    for (int i = 0; i < 4; ++i) {
+      __half2 h[kPairs];
+      mx_decode_word<XF>(v[i], h);
+#pragma unroll
+      for (int q = 0; q < kPairs; ++q) acc[i * kPairs + q] = ffma2(w, __half22float2(h[q]), acc[i * kPairs + q]);
+    }
   }
 }
 

@@ -6,6 +6,8 @@
 // an octet (eight consecutive samples of a unit), four lanes a block, so a
 // block's largest magnitude takes two shuffles and its codes leave as one
 // 8-byte (e2m1: 4-byte) store per lane.
+#include <initializer_list>
+
 #include "mx.cuh"
 
 namespace pxb {
@@ -28,26 +30,6 @@ template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
   return static_cast<float>(v);
 }
-
-// Eight consecutive values of a row, zero past `left`.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *__restrict__ p, int64_t step, int left, float (&v)[8]) {
-  if (VEC && left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4 *>(p);
-      const T *h = reinterpret_cast<const T *>(&a);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_f32(h[i]);
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32(p[i * step]) : 0.0f;
-}
-
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
@@ -57,24 +39,210 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T *__restrict__ p, int left, const float (&v)[8]) {
-  if (VEC && left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+// How a warp's 32 octets (its tile) lie in the rows.
+//
+// ALIGNED: octets of all rows in a line; a lane moves its octet in 16-byte
+// accesses (rows on 16-byte boundaries).
+// RUN, RUN2, TILE: rows at any element. An octet a lane would be eight
+// accesses 32 bytes apart, each touching every sector of the tile; instead the
+// warp moves the tile in runs of addresses -- lane l the elements l, l + 32,
+// ... -- and turns it into octets through its own kilobyte of shared memory.
+// RUN: a tile is 256 samples of one row; RUN2: the same in pairs of 16-bit
+// elements (rows on 4-byte boundaries); TILE: `width` blocks (1, 2 or 4) of 8 /
+// width rows, for rows of 128 samples at most.
+enum Layout { ALIGNED, RUN, RUN2, TILE };
+
+struct Grid {
+  int32_t rows, batch, nb, width;  // width: a tile's blocks a row (not ALIGNED)
+  FastDiv per_row;                 // ALIGNED: blocks a row; else tiles a row
+  uint32_t tiles;
+};
+
+struct Octet {
+  uint32_t u;   // row
+  int32_t b;    // first sample
+  int64_t at;   // index among all octets
+  bool on;      // within the rows
+};
+
+template <int LAYOUT>
+__device__ __forceinline__ Octet octet_of(const Grid &g, uint32_t tile, int lane) {
+  Octet o;
+  if constexpr (LAYOUT != ALIGNED) {
+    const uint32_t group = g.per_row.div(tile), seg = tile - group * g.per_row.d;
+    const int blk = lane >> 2, shift = LAYOUT == TILE ? 31 - __clz(g.width) : 3;
+    o.u = group * (8 >> shift) + (blk >> shift);
+    const int32_t k = (seg << shift) + (blk & ((1 << shift) - 1));
+    o.b = k * kMxBlock + (lane & 3) * 8;
+    o.on = o.u < static_cast<uint32_t>(g.rows) && k < g.nb;
+    o.at = (static_cast<int64_t>(o.u) * g.nb + k) * 4 + (lane & 3);
+  } else {
+    o.at = static_cast<int64_t>(tile) * 32 + lane;
+    const uint32_t blk = static_cast<uint32_t>(o.at >> 2);
+    o.u = g.per_row.div(blk);
+    o.b = static_cast<int32_t>(blk - o.u * g.per_row.d) * kMxBlock + (lane & 3) * 8;
+    o.on = o.at < static_cast<int64_t>(g.rows) * g.nb * 4;
+  }
+  return o;
+}
+
+// The move q of lane l in a tile: kEach neighbouring elements of row `u` from
+// sample `b` on; none where u is outside the rows.
+template <int LAYOUT>
+struct Moves {
+  static constexpr int kEach = LAYOUT == RUN2 ? 2 : 1, kMoves = 8 / kEach;
+  uint32_t u0;
+  int32_t b0;
+  int shift;  // TILE: log2 of the tile's blocks a row
+  __device__ __forceinline__ Moves(const Grid &g, uint32_t tile, int lane) {
+    const uint32_t group = g.per_row.div(tile), seg = tile - group * g.per_row.d;
+    shift = LAYOUT == TILE ? 31 - __clz(g.width) : 3;
+    u0 = group * (8 >> shift);
+    b0 = static_cast<int32_t>(seg) * 256 + lane * kEach;  // TILE has one tile a row
+  }
+  __device__ __forceinline__ uint32_t u(int q) const { return LAYOUT == TILE ? u0 + (q >> shift) : u0; }
+  __device__ __forceinline__ int32_t b(int q) const {
+    return LAYOUT == TILE ? b0 + (q & ((1 << shift) - 1)) * kMxBlock : b0 + q * 32 * kEach;
+  }
+};
+
+// What a lane has read of its tile, before it is turned into its octet: the
+// words as they came, so that nothing waits between the loads.
+template <typename T, int LAYOUT>
+struct Raw {
+  T v[8];
+};
+template <typename T>
+struct Raw<T, RUN2> {
+  uint32_t v[4];
+};
+template <typename T>
+struct Raw<T, ALIGNED> {
+  uint4 v[sizeof(T) / 2];
+  float tail[8];
+};
+
+// The lane's share of the tile from rows `su` elements apart; zero outside.
+// `keep(u)`: whether row u is read.
+template <typename T, int LAYOUT, typename Keep>
+__device__ __forceinline__ void fetch(const Grid &g, uint32_t tile, const Octet &o, const T *x, int64_t su, Keep keep,
+                                      Raw<T, LAYOUT> &r) {
+  if constexpr (LAYOUT == ALIGNED) {
+    const T *p = x + o.u * su + o.b;
+    if (o.on && o.b + 8 <= g.batch) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4 *>(p)[i];
     } else {
-      uint4 a;
-      T *h = reinterpret_cast<T *>(&a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.tail[i] = o.on && o.b + i < g.batch ? to_f32(p[i]) : 0.0f;
+    }
+  } else {
+    const Moves<LAYOUT> m(g, tile, threadIdx.x & 31);
+    if constexpr (LAYOUT == TILE) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t u = m.u(q);
+        const bool ok = u < static_cast<uint32_t>(g.rows) && m.b(q) < g.batch && keep(u);
+        r.v[q] = ok ? x[u * su + m.b(q)] : T(0.0f);
+      }
+    } else {
+      const int32_t end = m.u0 < static_cast<uint32_t>(g.rows) && keep(m.u0) ? g.batch : 0;
+      const T *p = x + m.u0 * su + m.b0;
+#pragma unroll
+      for (int q = 0; q < Moves<LAYOUT>::kMoves; ++q) {
+        if constexpr (LAYOUT == RUN) {
+          r.v[q] = m.b(q) < end ? p[q * 32] : T(0.0f);
+        } else {
+          r.v[q] = 0;
+          if (m.b(q) + 1 < end) r.v[q] = *reinterpret_cast<const uint32_t *>(p + q * 64);
+          else if (m.b(q) < end) r.v[q] = *reinterpret_cast<const uint16_t *>(p + q * 64);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int LAYOUT>
+__device__ __forceinline__ void settle(const Grid &g, const Octet &o, const Raw<T, LAYOUT> &r, float *buf,
+                                       float (&v)[8]) {
+  if constexpr (LAYOUT == ALIGNED) {
+    if (o.on && o.b + 8 <= g.batch) {
+      const T *h = reinterpret_cast<const T *>(r.v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = to_f32(h[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = r.tail[i];
+    }
+  } else {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < Moves<LAYOUT>::kMoves; ++q) {
+      if constexpr (LAYOUT == RUN2) {
+        const T *h = reinterpret_cast<const T *>(&r.v[q]);
+        reinterpret_cast<float2 *>(buf)[q * 32 + lane] = make_float2(to_f32(h[0]), to_f32(h[1]));
+      } else {
+        buf[q * 32 + lane] = to_f32(r.v[q]);
+      }
+    }
+    __syncwarp();
+    const float4 a = reinterpret_cast<const float4 *>(buf)[lane * 2], b = reinterpret_cast<const float4 *>(buf)[lane * 2 + 1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+}
+
+// The lane's octet out to rows `ld` elements apart. `keep(u)`: whether row u
+// is written.
+template <typename T, int LAYOUT, typename Keep>
+__device__ __forceinline__ void put(const Grid &g, uint32_t tile, const Octet &o, T *out, int64_t ld, Keep keep,
+                                    float *buf, const float (&v)[8]) {
+  if constexpr (LAYOUT != ALIGNED) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    reinterpret_cast<float4 *>(buf)[lane * 2] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(buf)[lane * 2 + 1] = make_float4(v[4], v[5], v[6], v[7]);
+    __syncwarp();
+    const Moves<LAYOUT> m(g, tile, lane);
+    if constexpr (LAYOUT == TILE) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t u = m.u(q);
+        if (u < static_cast<uint32_t>(g.rows) && m.b(q) < g.batch && keep(u)) out[u * ld + m.b(q)] = from_f32<T>(buf[q * 32 + lane]);
+      }
+    } else {
+      const int32_t end = m.u0 < static_cast<uint32_t>(g.rows) && keep(m.u0) ? g.batch : 0;
+      T *p = out + m.u0 * ld + m.b0;
+#pragma unroll
+      for (int q = 0; q < Moves<LAYOUT>::kMoves; ++q) {
+        if constexpr (LAYOUT == RUN) {
+          if (m.b(q) < end) p[q * 32] = from_f32<T>(buf[q * 32 + lane]);
+        } else {
+          const float2 two = reinterpret_cast<const float2 *>(buf)[q * 32 + lane];
+          uint32_t w;
+          T *h = reinterpret_cast<T *>(&w);
+          h[0] = from_f32<T>(two.x), h[1] = from_f32<T>(two.y);
+          if (m.b(q) + 1 < end) *reinterpret_cast<uint32_t *>(p + q * 64) = w;
+          else if (m.b(q) < end) p[q * 64] = h[0];
+        }
+      }
+    }
+  } else {
+    if (!o.on || !keep(o.u)) return;
+    T *p = out + o.u * ld + o.b;
+    if (o.b + 8 <= g.batch) {
+      uint4 a[sizeof(T) / 2];
+      T *h = reinterpret_cast<T *>(a);
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
-      *reinterpret_cast<uint4 *>(p) = a;
-    }
-    return;
-  }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < left) p[i] = from_f32<T>(v[i]);
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4 *>(p)[i] = a[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (o.b + i < g.batch) p[i] = from_f32<T>(v[i]);
+    }
+  }
 }
 
 // A lane's octet into its block's codes and scale (every lane of the warp
@@ -93,118 +261,204 @@ __device__ __forceinline__ void encode_octet(const float (&v)[8], bool keep, boo
   }
 }
 
-template <typename T, int FMT, bool VEC>
-__global__ void __launch_bounds__(256) mx_quantize_kernel(uint32_t blocks, FastDiv per_row, int32_t batch,
-                                                          const T *__restrict__ x, int64_t su, int64_t sb, bool keep,
-                                                          const int64_t *__restrict__ ids, int32_t num_units,
-                                                          uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
-  const int64_t octets = static_cast<int64_t>(blocks) * 4;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t o0 = blockIdx.x * static_cast<int64_t>(blockDim.x) + (threadIdx.x & ~31); o0 < octets; o0 += stride) {
-    int64_t o = o0 + (threadIdx.x & 31);
-    bool on = o < octets;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (on) {
-      const uint32_t blk = static_cast<uint32_t>(o >> 2), u = per_row.div(blk);
-      const int32_t b = static_cast<int32_t>(blk - u * per_row.d) * kMxBlock + static_cast<int32_t>(o & 3) * 8;
-      load8<T, VEC>(x + u * su + b * sb, sb, batch - b, v);
-      if (ids != nullptr) {
-        const int64_t row = ids[u];
-        on = row >= 0 && row < num_units;
-        o += (row - u) * (4 * static_cast<int64_t>(per_row.d));
-      }
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+struct All {
+  __device__ __forceinline__ bool operator()(uint32_t) const { return true; }
+};
+
+// Warps step through the tiles two at a time, so that two tiles' loads are in
+// flight together.
+#define PXB_MX_TILES(g)                                                                                 \
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;                                           \
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * kWarps;                                      \
+  for (uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * kWarps + warp; t0 < (g).tiles; t0 += 2 * step)
+
+template <typename T, int FMT, int LAYOUT>
+__global__ void __launch_bounds__(kThreads) mx_quantize_kernel(Grid g, const T *__restrict__ x, int64_t su, bool keep,
+                                                               const int64_t *__restrict__ ids,
+                                                               int32_t num_units, uint8_t *__restrict__ codes,
+                                                               uint8_t *__restrict__ scales) {
+  __shared__ __align__(16) float tiles[LAYOUT != ALIGNED ? kWarps : 1][256];
+  PXB_MX_TILES(g) {
+    Octet o[2];
+    Raw<T, LAYOUT> r[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint64_t t = t0 + k * step;
+      o[k] = octet_of<LAYOUT>(g, static_cast<uint32_t>(t), lane);
+      if (t >= g.tiles) o[k].on = false;
+      else fetch<T, LAYOUT>(g, static_cast<uint32_t>(t), o[k], x, su, All(), r[k]);
     }
-    encode_octet<FMT>(v, keep, on, o, codes, scales);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (t0 + k * step >= g.tiles) break;
+      float v[8];
+      settle<T, LAYOUT>(g, o[k], r[k], tiles[LAYOUT != ALIGNED ? warp : 0], v);
+      int64_t at = o[k].at;
+      bool on = o[k].on;
+      if (ids != nullptr && on) {
+        const int64_t row = ids[o[k].u];
+        on = row >= 0 && row < num_units;
+        at += (row - o[k].u) * (4 * static_cast<int64_t>(g.nb));
+      }
+      encode_octet<FMT>(v, keep, on, at, codes, scales);
+    }
   }
 }
 
-template <typename T, int FMT, bool VEC>
-__global__ void __launch_bounds__(256) mx_dequantize_kernel(uint32_t blocks, FastDiv per_row, int32_t batch,
-                                                            const uint8_t *__restrict__ codes,
-                                                            const uint8_t *__restrict__ scales, T *__restrict__ out,
-                                                            int64_t ld) {
-  const int64_t octets = static_cast<int64_t>(blocks) * 4;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t o = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; o < octets; o += stride) {
-    const uint32_t blk = static_cast<uint32_t>(o >> 2), u = per_row.div(blk);
-    const int32_t b = static_cast<int32_t>(blk - u * per_row.d) * kMxBlock + static_cast<int32_t>(o & 3) * 8;
-    const float s = mx_scale_value(scales[blk]);
-    float v[8];
-    mx_decode8<FMT>(mx_load8<FMT>(codes, o), v);
+// Samples at any stride. A lane takes a whole block of one unit, the lanes of
+// a warp 32 neighbouring units: a sample-major batch (units adjacent) is then
+// read in full lines, and the block's scale and codes need no other lane.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kThreads) mx_quantize_strided_kernel(int32_t rows, int32_t batch, int32_t nb,
+                                                                       FastDiv groups, const T *__restrict__ x,
+                                                                       int64_t su, int64_t sb, bool keep,
+                                                                       const int64_t *__restrict__ ids,
+                                                                       int32_t num_units, uint8_t *__restrict__ codes,
+                                                                       uint8_t *__restrict__ scales) {
+  const int lane = threadIdx.x & 31;
+  const uint64_t total = static_cast<uint64_t>(groups.d) * nb, step = static_cast<uint64_t>(gridDim.x) * kWarps;
+  for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < total; t += step) {
+    const uint32_t k = groups.div(static_cast<uint32_t>(t));
+    const int64_t u = static_cast<int64_t>(static_cast<uint32_t>(t) - k * groups.d) * 32 + lane;
+    if (u >= rows) continue;
+    const int32_t b = static_cast<int32_t>(k) * kMxBlock;
+    const T *p = x + u * su + b * sb;
+    float v[4][8];
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], s);
-    store8<T, VEC>(out + u * ld + b, batch - b, v);
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[q][i] = b + q * 8 + i < batch ? to_f32(p[(q * 8 + i) * sb]) : 0.0f;
+      m = max(m, mx_amax8(v[q]));
+    }
+    const int64_t row = ids != nullptr ? ids[u] : u;
+    if (row < 0 || row >= num_units) continue;
+    const uint32_t s = mx_scale_byte<FMT>(m);
+    const int64_t at = row * nb + k;
+    uint64_t c[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c[q] = mx_encode8<FMT>(v[q], s, keep);
+    uint4 *out = reinterpret_cast<uint4 *>(codes + at * mx_block_bytes<FMT>());
+    if constexpr (FMT == PXB_MX_E2M1) {
+      out[0] = make_uint4(c[0], c[1], c[2], c[3]);
+    } else {
+      out[0] = make_uint4(c[0], c[0] >> 32, c[1], c[1] >> 32);
+      out[1] = make_uint4(c[2], c[2] >> 32, c[3], c[3] >> 32);
+    }
+    scales[at] = static_cast<uint8_t>(s);
   }
 }
+
+template <typename T, int FMT, int LAYOUT>
+__global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(Grid g, const uint8_t *__restrict__ codes,
+                                                                 const uint8_t *__restrict__ scales, T *out,
+                                                                 int64_t ld) {
+  __shared__ __align__(16) float tiles[LAYOUT != ALIGNED ? kWarps : 1][256];
+  PXB_MX_TILES(g) {
+    Octet o[2];
+    uint64_t c[2] = {0, 0};
+    uint32_t s[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint64_t t = t0 + k * step;
+      o[k] = octet_of<LAYOUT>(g, static_cast<uint32_t>(t), lane);
+      if (t >= g.tiles) o[k].on = false;
+      if (o[k].on) {
+        c[k] = mx_load8<FMT>(codes, o[k].at);
+        s[k] = __ldg(scales + (o[k].at >> 2));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (t0 + k * step >= g.tiles) break;
+      float v[8];
+      mx_decode8<FMT>(c[k], v);
+      const float sc = mx_scale_value(s[k]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], sc);
+      put<T, LAYOUT>(g, static_cast<uint32_t>(t0 + k * step), o[k], out, ld, All(),
+                     tiles[LAYOUT != ALIGNED ? warp : 0], v);
+    }
+  }
+}
+
+// The units a masked pass works on, and whether it changes their rows.
+struct Mask {
+  const int32_t *__restrict__ level;
+  int32_t target;
+  const uint8_t *__restrict__ roles;
+  __device__ __forceinline__ bool here(uint32_t u) const { return level == nullptr || __ldg(level + u) == target; }
+  __device__ __forceinline__ uint8_t role(uint32_t u) const { return roles == nullptr ? 0 : __ldg(roles + u); }
+};
 
 // The forward's masked apply, in place, and the checkpoint of its result: the
-// units at `target` take act(acc); an input keeps its value. Both leave their
-// codes; no other row is read or written.
-template <int FMT, bool VEC>
-__global__ void __launch_bounds__(256) mx_unit_apply_kernel(uint32_t blocks, FastDiv per_row, int32_t batch,
-                                                            int32_t act_kind, float *__restrict__ rows,
-                                                            const int32_t *__restrict__ level, int32_t target,
-                                                            const uint8_t *__restrict__ roles,
-                                                            uint8_t *__restrict__ codes,
-                                                            uint8_t *__restrict__ scales) {
-  const int64_t octets = static_cast<int64_t>(blocks) * 4;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t o0 = blockIdx.x * static_cast<int64_t>(blockDim.x) + (threadIdx.x & ~31); o0 < octets; o0 += stride) {
-    const int64_t o = o0 + (threadIdx.x & 31);
-    bool on = o < octets;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (on) {
-      const uint32_t blk = static_cast<uint32_t>(o >> 2), u = per_row.div(blk);
-      on = level == nullptr || level[u] == target;
-      if (on) {
-        const int32_t b = static_cast<int32_t>(blk - u * per_row.d) * kMxBlock + static_cast<int32_t>(o & 3) * 8;
-        float *p = rows + static_cast<int64_t>(u) * batch + b;
-        load8<float, VEC>(p, 1, batch - b, v);
-        const uint8_t role = roles != nullptr ? roles[u] : 0;
-        if (role != 1) {
-          const int kind = unit_act_kind(act_kind, role);
+// units at the mask's level take act(rows); an input keeps its row. Both leave
+// their codes; no other row is read or written.
+template <int FMT, int LAYOUT>
+__global__ void __launch_bounds__(kThreads) mx_unit_apply_kernel(Grid g, int32_t act_kind, float *rows, Mask m,
+                                                                 uint8_t *__restrict__ codes,
+                                                                 uint8_t *__restrict__ scales) {
+  __shared__ __align__(16) float tiles[LAYOUT != ALIGNED ? kWarps : 1][256];
+  const auto here = [&](uint32_t u) { return m.here(u); };
+  const auto moves = [&](uint32_t u) { return m.here(u) && m.role(u) != 1; };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float *buf = tiles[LAYOUT != ALIGNED ? warp : 0];
+  for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kWarps + warp; t < g.tiles;
+       t += static_cast<uint64_t>(gridDim.x) * kWarps) {
+    Octet o = octet_of<LAYOUT>(g, static_cast<uint32_t>(t), lane);
+    o.on = o.on && m.here(o.u);
+    if (!__any_sync(0xffffffffu, o.on)) continue;
+    Raw<float, LAYOUT> r;
+    fetch<float, LAYOUT>(g, static_cast<uint32_t>(t), o, rows, g.batch, here, r);
+    float v[8];
+    settle<float, LAYOUT>(g, o, r, buf, v);
+    if (o.on) {
+      const uint8_t role = m.role(o.u);
+      if (role != 1) {
+        const int kind = unit_act_kind(act_kind, role);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = i < batch - b ? act_fn(kind, v[i]) : 0.0f;
-          store8<float, VEC>(p, batch - b, v);
-        }
+        for (int i = 0; i < 8; ++i) v[i] = o.b + i < g.batch ? act_fn(kind, v[i]) : 0.0f;
       }
     }
-    encode_octet<FMT>(v, true, on, o, codes, scales);
+    put<float, LAYOUT>(g, static_cast<uint32_t>(t), o, rows, g.batch, moves, buf, v);
+    encode_octet<FMT>(v, true, o.on, o.at, codes, scales);
   }
 }
 
 // out = (acc + seed) * act'(checkpointed activation).
-template <int FMT, bool VEC>
-__global__ void __launch_bounds__(256) mx_unit_grad_kernel(uint32_t blocks, FastDiv per_row, int32_t batch,
-                                                           int32_t act_kind, const float *acc, const float *seed,
-                                                           const uint8_t *__restrict__ codes,
-                                                           const uint8_t *__restrict__ scales,
-                                                           const int32_t *__restrict__ level, int32_t target,
-                                                           const uint8_t *__restrict__ roles, float *out) {
-  const int64_t octets = static_cast<int64_t>(blocks) * 4;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t o = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; o < octets; o += stride) {
-    const uint32_t blk = static_cast<uint32_t>(o >> 2), u = per_row.div(blk);
-    if (level != nullptr && level[u] != target) continue;
-    const uint8_t role = roles != nullptr ? roles[u] : 0;
-    if (role == 1) continue;
-    const int32_t b = static_cast<int32_t>(blk - u * per_row.d) * kMxBlock + static_cast<int32_t>(o & 3) * 8;
-    if (b >= batch) continue;
-    const int kind = unit_act_kind(act_kind, role);
-    const int64_t at = static_cast<int64_t>(u) * batch + b;
-    float a[8], g[8];
-    load8<float, VEC>(acc + at, 1, batch - b, g);
+template <int FMT, int LAYOUT>
+__global__ void __launch_bounds__(kThreads, 4) mx_unit_grad_kernel(Grid g, int32_t act_kind, const float *acc,
+                                                                const float *seed, const uint8_t *__restrict__ codes,
+                                                                const uint8_t *__restrict__ scales, Mask m,
+                                                                float *out) {
+  __shared__ __align__(16) float tiles[LAYOUT != ALIGNED ? kWarps : 1][256];
+  const auto moves = [&](uint32_t u) { return m.here(u) && m.role(u) != 1; };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float *buf = tiles[LAYOUT != ALIGNED ? warp : 0];
+  for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kWarps + warp; t < g.tiles;
+       t += static_cast<uint64_t>(gridDim.x) * kWarps) {
+    Octet o = octet_of<LAYOUT>(g, static_cast<uint32_t>(t), lane);
+    const uint8_t role = o.on ? m.role(o.u) : 1;
+    o.on = o.on && role != 1 && m.here(o.u);
+    if (!__any_sync(0xffffffffu, o.on)) continue;
+    Raw<float, LAYOUT> ra, rs;
+    fetch<float, LAYOUT>(g, static_cast<uint32_t>(t), o, acc, g.batch, moves, ra);
+    if (seed != nullptr) fetch<float, LAYOUT>(g, static_cast<uint32_t>(t), o, seed, g.batch, moves, rs);
+    const uint64_t c = o.on ? mx_load8<FMT>(codes, o.at) : 0;
+    const float sc = mx_scale_value(o.on ? __ldg(scales + (o.at >> 2)) : 0);
+    float v[8], a[8];
+    settle<float, LAYOUT>(g, o, ra, buf, v);
     if (seed != nullptr) {
-      float sd[8];
-      load8<float, VEC>(seed + at, 1, batch - b, sd);
+      settle<float, LAYOUT>(g, o, rs, buf, a);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = __fadd_rn(g[i], sd[i]);
+      for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], a[i]);
     }
-    mx_decode8<FMT>(mx_load8<FMT>(codes, o), a);
-    const float s = mx_scale_value(scales[blk]);
+    const int kind = unit_act_kind(act_kind, role);
+    mx_decode8<FMT>(c, a);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = __fmul_rn(g[i], act_prime_from_act(kind, __fmul_rn(a[i], s)));
-    store8<float, VEC>(out + at, batch - b, g);
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], act_prime_from_act(kind, __fmul_rn(a[i], sc)));
+    put<float, LAYOUT>(g, static_cast<uint32_t>(t), o, out, g.batch, moves, buf, v);
   }
 }
 
@@ -218,9 +472,29 @@ static int check_rows(const char *fn, int32_t num_units, int32_t batch, int fmt,
   return PXB_OK;
 }
 
-static bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+// The layout for rows `ld` elements of `size` bytes apart from p (any of a
+// pass's row buffers: the first that is off the boundary decides).
+static int layout_of(int32_t batch, int size, std::initializer_list<const void *> ps, int64_t ld) {
+  uintptr_t bits = static_cast<uintptr_t>(ld * size);
+  for (const void *p : ps) bits |= reinterpret_cast<uintptr_t>(p);
+  if ((bits & 15) == 0) return ALIGNED;
+  if (batch <= 4 * kMxBlock) return TILE;
+  return size == 2 && (bits & 3) == 0 ? RUN2 : RUN;
+}
 
-// One instance of the statements per format (F) / element type (T).
+static Grid grid_of(int32_t rows, int32_t batch, int layout) {
+  const int32_t nb = static_cast<int32_t>(mx_blocks(batch));
+  if (layout == ALIGNED)
+    return Grid{rows, batch, nb, 0, FastDiv(static_cast<uint32_t>(nb)),
+                static_cast<uint32_t>((static_cast<int64_t>(rows) * nb + 7) / 8)};
+  const int32_t width = layout != TILE ? 8 : nb <= 1 ? 1 : nb <= 2 ? 2 : 4, segs = (nb + width - 1) / width;
+  const int64_t groups = (static_cast<int64_t>(rows) * width + 7) / 8;
+  return Grid{rows, batch, nb, width, FastDiv(static_cast<uint32_t>(segs)), static_cast<uint32_t>(groups * segs)};
+}
+
+static int ctas_for(const Grid &g, int per_sm) { return grid_for(g.tiles, kWarps, per_sm); }
+
+// One instance of the statements per format (F), element type (T), layout (L).
 #define PXB_MX_FMT8(FMT, ...)                                                       \
   do {                                                                              \
     if ((FMT) == PXB_MX_E4M3) { constexpr int F = PXB_MX_E4M3; __VA_ARGS__; }        \
@@ -236,6 +510,17 @@ static bool aligned(const void *p, int bytes) { return (reinterpret_cast<uintptr
     if ((DT) == PXB_DT_F32) { using T = float; __VA_ARGS__; }                        \
     else if ((DT) == PXB_DT_BF16) { using T = __nv_bfloat16; __VA_ARGS__; }          \
     else { using T = __half; __VA_ARGS__; }                                          \
+  } while (0)
+#define PXB_MX_ROWS(LAY, ...)                                                       \
+  do {                                                                              \
+    if ((LAY) == ALIGNED) { constexpr int L = ALIGNED; __VA_ARGS__; }                \
+    else if ((LAY) == TILE) { constexpr int L = TILE; __VA_ARGS__; }                 \
+    else { constexpr int L = RUN; __VA_ARGS__; }                                     \
+  } while (0)
+#define PXB_MX_ROWS2(LAY, ...)                                                      \
+  do {                                                                              \
+    if (sizeof(T) == 2 && (LAY) == RUN2) { constexpr int L = sizeof(T) == 2 ? RUN2 : RUN; __VA_ARGS__; } \
+    else PXB_MX_ROWS(LAY, __VA_ARGS__);                                              \
   } while (0)
 
 }  // namespace pxb
@@ -253,18 +538,25 @@ extern "C" int pxb_mx_quantize(int32_t num_rows, int32_t batch, const void *x, i
   PXB_REQUIRE(dtype >= PXB_DT_F32 && dtype <= PXB_DT_F16, "pxb_mx_quantize: unknown type %d", dtype);
   if (blocks == 0) return PXB_OK;
   PXB_REQUIRE(x && codes && scales, "pxb_mx_quantize: a pointer is NULL");
-  PXB_REQUIRE(aligned(codes, 16), "pxb_mx_quantize: codes must be 16-byte aligned");
+  PXB_REQUIRE(aligned16(codes), "pxb_mx_quantize: codes must be 16-byte aligned");
   const int size = dtype == PXB_DT_F32 ? 4 : 2;
-  const bool vec = stride_sample == 1 && aligned16(x) && (stride_row * size) % 16 == 0;
-  const FastDiv per_row(static_cast<uint32_t>(mx_blocks(batch)));
-  const int grid = grid_for(blocks * 4, 256, 16);
   cudaStream_t st = as_stream(stream);
-  const uint32_t nb = static_cast<uint32_t>(blocks);
-  PXB_MX_DTYPE(dtype, PXB_MX_FMT(fmt, {
-    const T *xt = static_cast<const T *>(x);
-    if (vec) mx_quantize_kernel<T, F, true><<<grid, 256, 0, st>>>(nb, per_row, batch, xt, stride_row, stride_sample, keep_nonzero != 0, ids, num_units, codes, scales);
-    else mx_quantize_kernel<T, F, false><<<grid, 256, 0, st>>>(nb, per_row, batch, xt, stride_row, stride_sample, keep_nonzero != 0, ids, num_units, codes, scales);
-  }));
+  if (stride_sample != 1 && batch > 1) {
+    const FastDiv groups(static_cast<uint32_t>((static_cast<int64_t>(num_rows) + 31) / 32));
+    const int32_t nb = static_cast<int32_t>(mx_blocks(batch));
+    const int ctas = grid_for(static_cast<int64_t>(groups.d) * nb, kWarps, 8);
+    PXB_MX_DTYPE(dtype, PXB_MX_FMT(fmt, {
+      mx_quantize_strided_kernel<T, F><<<ctas, kThreads, 0, st>>>(num_rows, batch, nb, groups, static_cast<const T *>(x),
+                                                                  stride_row, stride_sample, keep_nonzero != 0, ids, num_units, codes, scales);
+    }));
+    PXB_LAUNCHED("mx_quantize_strided_kernel");
+    return PXB_OK;
+  }
+  const int layout = layout_of(batch, size, {x}, stride_row);
+  const Grid g = grid_of(num_rows, batch, layout);
+  PXB_MX_DTYPE(dtype, PXB_MX_FMT(fmt, PXB_MX_ROWS2(layout, {
+    mx_quantize_kernel<T, F, L><<<ctas_for(g, 8), kThreads, 0, st>>>(g, static_cast<const T *>(x), stride_row, keep_nonzero != 0, ids, num_units, codes, scales);
+  })));
   PXB_LAUNCHED("mx_quantize_kernel");
   return PXB_OK;
 }
@@ -277,18 +569,14 @@ extern "C" int pxb_mx_dequantize(int32_t num_units, int32_t batch, const uint8_t
   PXB_REQUIRE(ld >= batch, "pxb_mx_dequantize: rows overlap");
   if (blocks == 0) return PXB_OK;
   PXB_REQUIRE(codes && scales && out, "pxb_mx_dequantize: a pointer is NULL");
-  PXB_REQUIRE(aligned(codes, 16), "pxb_mx_dequantize: codes must be 16-byte aligned");
+  PXB_REQUIRE(aligned16(codes), "pxb_mx_dequantize: codes must be 16-byte aligned");
   const int size = dtype == PXB_DT_F32 ? 4 : 2;
-  const bool vec = aligned16(out) && (ld * size) % 16 == 0;
-  const FastDiv per_row(static_cast<uint32_t>(mx_blocks(batch)));
-  const int grid = grid_for(blocks * 4, 256, 16);
+  const int layout = layout_of(batch, size, {out}, ld);
+  const Grid g = grid_of(num_units, batch, layout);
   cudaStream_t st = as_stream(stream);
-  const uint32_t nb = static_cast<uint32_t>(blocks);
-  PXB_MX_DTYPE(dtype, PXB_MX_FMT(fmt, {
-    T *ot = static_cast<T *>(out);
-    if (vec) mx_dequantize_kernel<T, F, true><<<grid, 256, 0, st>>>(nb, per_row, batch, codes, scales, ot, ld);
-    else mx_dequantize_kernel<T, F, false><<<grid, 256, 0, st>>>(nb, per_row, batch, codes, scales, ot, ld);
-  }));
+  PXB_MX_DTYPE(dtype, PXB_MX_FMT(fmt, PXB_MX_ROWS2(layout, {
+    mx_dequantize_kernel<T, F, L><<<ctas_for(g, 8), kThreads, 0, st>>>(g, codes, scales, static_cast<T *>(out), ld);
+  })));
   PXB_LAUNCHED("mx_dequantize_kernel");
   return PXB_OK;
 }
@@ -302,16 +590,13 @@ extern "C" int pxb_mx_unit_apply(int32_t num_units, int32_t batch, int32_t act_k
   PXB_REQUIRE(act_code_ok(act_kind), "pxb_mx_unit_apply: unknown activation code %d", act_kind);
   if (blocks == 0) return PXB_OK;
   PXB_REQUIRE(rows && codes && scales, "pxb_mx_unit_apply: a pointer is NULL");
-  PXB_REQUIRE(aligned(codes, 16), "pxb_mx_unit_apply: codes must be 16-byte aligned");
-  const bool vec = aligned16(rows) && batch % 4 == 0;
-  const FastDiv per_row(static_cast<uint32_t>(mx_blocks(batch)));
-  const int grid = grid_for(blocks * 4, 256, 8);
+  PXB_REQUIRE(aligned16(codes), "pxb_mx_unit_apply: codes must be 16-byte aligned");
+  const int layout = layout_of(batch, 4, {rows}, batch);
+  const Grid g = grid_of(num_units, batch, layout);
   cudaStream_t st = as_stream(stream);
-  const uint32_t nb = static_cast<uint32_t>(blocks);
-  PXB_MX_FMT8(fmt, {
-    if (vec) mx_unit_apply_kernel<F, true><<<grid, 256, 0, st>>>(nb, per_row, batch, act_kind, rows, level, target_level, roles, codes, scales);
-    else mx_unit_apply_kernel<F, false><<<grid, 256, 0, st>>>(nb, per_row, batch, act_kind, rows, level, target_level, roles, codes, scales);
-  });
+  PXB_MX_FMT8(fmt, PXB_MX_ROWS(layout, {
+    mx_unit_apply_kernel<F, L><<<ctas_for(g, 8), kThreads, 0, st>>>(g, act_kind, rows, Mask{level, target_level, roles}, codes, scales);
+  }));
   PXB_LAUNCHED("mx_unit_apply_kernel");
   return PXB_OK;
 }
@@ -326,16 +611,13 @@ extern "C" int pxb_mx_unit_grad(int32_t num_units, int32_t batch, int32_t act_ki
   PXB_REQUIRE(act_code_ok(act_kind), "pxb_mx_unit_grad: unknown activation code %d", act_kind);
   if (blocks == 0) return PXB_OK;
   PXB_REQUIRE(acc && codes && scales && out, "pxb_mx_unit_grad: a pointer is NULL");
-  PXB_REQUIRE(aligned(codes, 16), "pxb_mx_unit_grad: codes must be 16-byte aligned");
-  const bool vec = aligned16(acc) && aligned16(out) && (seed == nullptr || aligned16(seed)) && batch % 4 == 0;
-  const FastDiv per_row(static_cast<uint32_t>(mx_blocks(batch)));
-  const int grid = grid_for(blocks * 4, 256, 16);
+  PXB_REQUIRE(aligned16(codes), "pxb_mx_unit_grad: codes must be 16-byte aligned");
+  const int layout = layout_of(batch, 4, {acc, seed, out}, batch);
+  const Grid g = grid_of(num_units, batch, layout);
   cudaStream_t st = as_stream(stream);
-  const uint32_t nb = static_cast<uint32_t>(blocks);
-  PXB_MX_FMT8(fmt, {
-    if (vec) mx_unit_grad_kernel<F, true><<<grid, 256, 0, st>>>(nb, per_row, batch, act_kind, acc, seed, codes, scales, level, target_level, roles, out);
-    else mx_unit_grad_kernel<F, false><<<grid, 256, 0, st>>>(nb, per_row, batch, act_kind, acc, seed, codes, scales, level, target_level, roles, out);
-  });
+  PXB_MX_FMT8(fmt, PXB_MX_ROWS(layout, {
+    mx_unit_grad_kernel<F, L><<<ctas_for(g, 8), kThreads, 0, st>>>(g, act_kind, acc, seed, codes, scales, Mask{level, target_level, roles}, out);
+  }));
   PXB_LAUNCHED("mx_unit_grad_kernel");
   return PXB_OK;
 }

@@ -74,28 +74,42 @@ template <int FMT>
 __device__ __forceinline__ uint64_t mx_encode8(const float (&x)[8], uint32_t scale, bool keep) {
   if (scale == 255u) return 0;
   const float inv = mx_inverse_scale(scale);
-  uint64_t out = 0;
+  float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const float2 y = make_float2(__fmul_rn(x[i], inv), __fmul_rn(x[i + 1], inv));
-    uint32_t c;
-    if constexpr (FMT == PXB_MX_E2M1) {
-      c = __nv_cvt_float2_to_fp4x2(y, __NV_E2M1, cudaRoundNearest);
-      if (keep) {
-        if (x[i] != 0.0f && (c & 0x07u) == 0) c |= 0x01u;
-        if (x[i + 1] != 0.0f && (c & 0x70u) == 0) c |= 0x10u;
-      }
-      out |= static_cast<uint64_t>(c & 0xffu) << (4 * i);
+  for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(x[i], inv);
+  uint32_t lo, hi = 0;
+  if constexpr (FMT == PXB_MX_E2M1) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\tcvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(lo) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+    if (keep) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (x[i] != 0.0f && (lo & (0x7u << (4 * i))) == 0) lo |= 0x1u << (4 * i);
+    }
+  } else {
+#define PXB_MX_ENCODE4(KIND, OUT, AT)                                                                            \
+  asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite." KIND "x2.f32 a, %2, %1;\n\tcvt.rn.satfinite." KIND         \
+      "x2.f32 b, %4, %3;\n\tmov.b32 %0, {a, b};\n\t}"                                                          \
+      : "=r"(OUT) : "f"(y[AT]), "f"(y[AT + 1]), "f"(y[AT + 2]), "f"(y[AT + 3]))
+    if constexpr (FMT == PXB_MX_E4M3) {
+      PXB_MX_ENCODE4("e4m3", lo, 0);
+      PXB_MX_ENCODE4("e4m3", hi, 4);
     } else {
-      c = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, FMT == PXB_MX_E4M3 ? __NV_E4M3 : __NV_E5M2);
-      if (keep) {
-        if (x[i] != 0.0f && (c & 0x007fu) == 0) c |= 0x0001u;
-        if (x[i + 1] != 0.0f && (c & 0x7f00u) == 0) c |= 0x0100u;
+      PXB_MX_ENCODE4("e5m2", lo, 0);
+      PXB_MX_ENCODE4("e5m2", hi, 4);
+    }
+#undef PXB_MX_ENCODE4
+    if (keep) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (x[i] != 0.0f && (lo & (0x7fu << (8 * i))) == 0) lo |= 0x1u << (8 * i);
+        if (x[i + 4] != 0.0f && (hi & (0x7fu << (8 * i))) == 0) hi |= 0x1u << (8 * i);
       }
-      out |= static_cast<uint64_t>(c & 0xffffu) << (8 * i);
     }
   }
-  return out;
+  return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
 // Four bytes of codes (4 in 8 bits, 8 in e2m1) -> pairs of values before the
@@ -159,6 +173,18 @@ __device__ __forceinline__ uint32_t mx_amax8(const float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
   return m;
+}
+
+// CTAs for a kernel whose CTAs step through `items`, `per_cta` at a time: one
+// full wave at most (a grid of 8 an SM where 6 fit would leave a second wave a
+// third full).
+template <auto KERNEL>
+inline int mx_grid(int64_t items, int per_cta, int threads) {
+  static const int resident = [threads] {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0) == cudaSuccess && n > 0 ? n : 1;
+  }();
+  return grid_for(items, per_cta, resident);
 }
 
 __host__ inline bool mx_format_ok(int fmt) { return fmt >= PXB_MX_E4M3 && fmt <= PXB_MX_E2M1; }

@@ -153,10 +153,13 @@ __device__ __forceinline__ void fetch(const Grid &g, uint32_t tile, const Octet 
         if constexpr (LAYOUT == RUN) {
           r.v[q] = m.b(q) < end ? p[q * 32] : T(0.0f);
         } else {
-          r.v[q] = 0;
-          if (m.b(q) + 1 < end) r.v[q] = *reinterpret_cast<const uint32_t *>(p + q * 64);
-          else if (m.b(q) < end) r.v[q] = *reinterpret_cast<const uint16_t *>(p + q * 64);
+          r.v[q] = m.b(q) < (end & ~1) ? *reinterpret_cast<const uint32_t *>(p + q * 64) : 0u;
         }
+      }
+      if (LAYOUT == RUN2 && (end & 1)) {  // the sample without a partner
+#pragma unroll
+        for (int q = 0; q < Moves<LAYOUT>::kMoves; ++q)
+          if (m.b(q) == end - 1) r.v[q] = *reinterpret_cast<const uint16_t *>(p + q * 64);
       }
     }
   }
@@ -222,22 +225,37 @@ __device__ __forceinline__ void put(const Grid &g, uint32_t tile, const Octet &o
           uint32_t w;
           T *h = reinterpret_cast<T *>(&w);
           h[0] = from_f32<T>(two.x), h[1] = from_f32<T>(two.y);
-          if (m.b(q) + 1 < end) *reinterpret_cast<uint32_t *>(p + q * 64) = w;
-          else if (m.b(q) < end) p[q * 64] = h[0];
+          if (m.b(q) < (end & ~1)) *reinterpret_cast<uint32_t *>(p + q * 64) = w;
+          if ((end & 1) && m.b(q) == end - 1) p[q * 64] = h[0];
         }
       }
     }
   } else {
-    if (!o.on || !keep(o.u)) return;
+    const bool on = o.on && keep(o.u);
     T *p = out + o.u * ld + o.b;
-    if (o.b + 8 <= g.batch) {
-      uint4 a[sizeof(T) / 2];
-      T *h = reinterpret_cast<T *>(a);
+    if constexpr (sizeof(T) == 4) {
+      // two lanes swap halves of their octets, so that each store instruction writes whole sectors: the first the even
+      // lanes' octets, the second the odd lanes'
+      const int lane = threadIdx.x & 31;
+      const bool odd = lane & 1, full = on && o.b + 8 <= g.batch;
+      const unsigned fulls = __ballot_sync(0xffffffffu, full);
+      float4 got;
+      got.x = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[4], 1);
+      got.y = __shfl_xor_sync(0xffffffffu, odd ? v[1] : v[5], 1);
+      got.z = __shfl_xor_sync(0xffffffffu, odd ? v[2] : v[6], 1);
+      got.w = __shfl_xor_sync(0xffffffffu, odd ? v[3] : v[7], 1);
+      if (fulls >> (lane & ~1) & 1) *reinterpret_cast<float4 *>(odd ? p - 4 : p) = odd ? got : make_float4(v[0], v[1], v[2], v[3]);
+      if (fulls >> (lane | 1) & 1) *reinterpret_cast<float4 *>(odd ? p + 4 : p + 8) = odd ? make_float4(v[4], v[5], v[6], v[7]) : got;
+      if (full) return;
+    } else if (on && o.b + 8 <= g.batch) {
+      uint4 a;
+      T *h = reinterpret_cast<T *>(&a);
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4 *>(p)[i] = a[i];
-    } else {
+      *reinterpret_cast<uint4 *>(p) = a;
+      return;
+    }
+    if (on) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (o.b + i < g.batch) p[i] = from_f32<T>(v[i]);
@@ -492,8 +510,6 @@ static Grid grid_of(int32_t rows, int32_t batch, int layout) {
   return Grid{rows, batch, nb, width, FastDiv(static_cast<uint32_t>(segs)), static_cast<uint32_t>(groups * segs)};
 }
 
-static int ctas_for(const Grid &g, int per_sm) { return grid_for(g.tiles, kWarps, per_sm); }
-
 // One instance of the statements per format (F), element type (T), layout (L).
 #define PXB_MX_FMT8(FMT, ...)                                                       \
   do {                                                                              \
@@ -544,9 +560,8 @@ extern "C" int pxb_mx_quantize(int32_t num_rows, int32_t batch, const void *x, i
   if (stride_sample != 1 && batch > 1) {
     const FastDiv groups(static_cast<uint32_t>((static_cast<int64_t>(num_rows) + 31) / 32));
     const int32_t nb = static_cast<int32_t>(mx_blocks(batch));
-    const int ctas = grid_for(static_cast<int64_t>(groups.d) * nb, kWarps, 8);
     PXB_MX_DTYPE(dtype, PXB_MX_FMT(fmt, {
-      mx_quantize_strided_kernel<T, F><<<ctas, kThreads, 0, st>>>(num_rows, batch, nb, groups, static_cast<const T *>(x),
+      mx_quantize_strided_kernel<T, F><<<mx_grid<mx_quantize_strided_kernel<T, F>>(static_cast<int64_t>(groups.d) * nb, kWarps, kThreads), kThreads, 0, st>>>(num_rows, batch, nb, groups, static_cast<const T *>(x),
                                                                   stride_row, stride_sample, keep_nonzero != 0, ids, num_units, codes, scales);
     }));
     PXB_LAUNCHED("mx_quantize_strided_kernel");
@@ -555,7 +570,7 @@ extern "C" int pxb_mx_quantize(int32_t num_rows, int32_t batch, const void *x, i
   const int layout = layout_of(batch, size, {x}, stride_row);
   const Grid g = grid_of(num_rows, batch, layout);
   PXB_MX_DTYPE(dtype, PXB_MX_FMT(fmt, PXB_MX_ROWS2(layout, {
-    mx_quantize_kernel<T, F, L><<<ctas_for(g, 8), kThreads, 0, st>>>(g, static_cast<const T *>(x), stride_row, keep_nonzero != 0, ids, num_units, codes, scales);
+    mx_quantize_kernel<T, F, L><<<mx_grid<mx_quantize_kernel<T, F, L>>(g.tiles, kWarps, kThreads), kThreads, 0, st>>>(g, static_cast<const T *>(x), stride_row, keep_nonzero != 0, ids, num_units, codes, scales);
   })));
   PXB_LAUNCHED("mx_quantize_kernel");
   return PXB_OK;
@@ -575,7 +590,7 @@ extern "C" int pxb_mx_dequantize(int32_t num_units, int32_t batch, const uint8_t
   const Grid g = grid_of(num_units, batch, layout);
   cudaStream_t st = as_stream(stream);
   PXB_MX_DTYPE(dtype, PXB_MX_FMT(fmt, PXB_MX_ROWS2(layout, {
-    mx_dequantize_kernel<T, F, L><<<ctas_for(g, 8), kThreads, 0, st>>>(g, codes, scales, static_cast<T *>(out), ld);
+    mx_dequantize_kernel<T, F, L><<<mx_grid<mx_dequantize_kernel<T, F, L>>(g.tiles, kWarps, kThreads), kThreads, 0, st>>>(g, codes, scales, static_cast<T *>(out), ld);
   })));
   PXB_LAUNCHED("mx_dequantize_kernel");
   return PXB_OK;
@@ -595,7 +610,7 @@ extern "C" int pxb_mx_unit_apply(int32_t num_units, int32_t batch, int32_t act_k
   const Grid g = grid_of(num_units, batch, layout);
   cudaStream_t st = as_stream(stream);
   PXB_MX_FMT8(fmt, PXB_MX_ROWS(layout, {
-    mx_unit_apply_kernel<F, L><<<ctas_for(g, 8), kThreads, 0, st>>>(g, act_kind, rows, Mask{level, target_level, roles}, codes, scales);
+    mx_unit_apply_kernel<F, L><<<mx_grid<mx_unit_apply_kernel<F, L>>(g.tiles, kWarps, kThreads), kThreads, 0, st>>>(g, act_kind, rows, Mask{level, target_level, roles}, codes, scales);
   }));
   PXB_LAUNCHED("mx_unit_apply_kernel");
   return PXB_OK;
@@ -616,7 +631,7 @@ extern "C" int pxb_mx_unit_grad(int32_t num_units, int32_t batch, int32_t act_ki
   const Grid g = grid_of(num_units, batch, layout);
   cudaStream_t st = as_stream(stream);
   PXB_MX_FMT8(fmt, PXB_MX_ROWS(layout, {
-    mx_unit_grad_kernel<F, L><<<ctas_for(g, 8), kThreads, 0, st>>>(g, act_kind, acc, seed, codes, scales, Mask{level, target_level, roles}, out);
+    mx_unit_grad_kernel<F, L><<<mx_grid<mx_unit_grad_kernel<F, L>>(g.tiles, kWarps, kThreads), kThreads, 0, st>>>(g, act_kind, acc, seed, codes, scales, Mask{level, target_level, roles}, out);
   }));
   PXB_LAUNCHED("mx_unit_grad_kernel");
   return PXB_OK;

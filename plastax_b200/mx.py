@@ -55,17 +55,29 @@ def _format(fmt: str, allowed=FORMATS, what: str = "format") -> int:
 
 
 def _on(dev: torch.device):
-    """The tensors' device as the current one for a call."""
+    """The tensors' device as the current one."""
     if dev.type != "cuda":
         raise ValueError("engine tensors must live on a CUDA device")
-    if dev.index is None or dev.index == torch.cuda.current_device():
+    if dev.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(dev)
+
+
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """Call an entry point on `dev` and its current stream."""
+    if dev.type == "cuda" and dev.index == torch.cuda.current_device():
+        call(name, *args, K._stream())
+        return
+    with _on(dev):
+        call(name, *args, K._stream())
 
 
 def _tensor(t, dtype, shape, what: str, dev: torch.device | None = None) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
+    if t.dtype is dtype and (shape is None or t.shape == shape) and t.is_contiguous() and (
+            dev is None or t.device == dev):
+        return t
     if t.dtype != dtype:
         raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
     if shape is not None and tuple(t.shape) != tuple(shape):
@@ -120,10 +132,14 @@ class MxRows:
     def empty(cls, num_units: int, batch: int, fmt: str, device, *, zero: bool = False) -> "MxRows":
         """Rows without values (`zero`: rows that read 0)."""
         _format(fmt)
+        if not 0 <= batch <= _MAX_BATCH:
+            raise ValueError(f"MxRows: batch must be in [0, {_MAX_BATCH}], got {batch}")
         new = torch.zeros if zero else torch.empty
         nb = num_blocks(batch)
-        return cls(new((num_units, nb * block_bytes(fmt)), dtype=torch.uint8, device=device),
-                   new((num_units, nb), dtype=torch.uint8, device=device), fmt, batch)
+        rows = object.__new__(cls)  # nothing to check in what is made here
+        rows.__dict__.update(codes=new((num_units, nb * block_bytes(fmt)), dtype=torch.uint8, device=device),
+                             scales=new((num_units, nb), dtype=torch.uint8, device=device), fmt=fmt, batch=batch)
+        return rows
 
 
 def mx_quantize(x: torch.Tensor, fmt: str, *, keep_nonzero: bool = False, ids: torch.Tensor | None = None,
@@ -148,10 +164,8 @@ def mx_quantize(x: torch.Tensor, fmt: str, *, keep_nonzero: bool = False, ids: t
                          f"expected {n} x {b} {fmt} on {x.device}")
     if ids is not None:
         _tensor(ids, torch.int64, (n,), "mx_quantize: ids", x.device)
-    with _on(x.device):
-        call("pxb_mx_quantize", n, b, x.data_ptr(), _DT[x.dtype], x.stride(0), x.stride(1), code,
-             1 if keep_nonzero else 0, K.ptr(ids), out.num_units, out.codes.data_ptr(), out.scales.data_ptr(),
-             K._stream())
+    _launch(x.device, "pxb_mx_quantize", n, b, x.data_ptr(), _DT[x.dtype], x.stride(0), x.stride(1), code,
+            1 if keep_nonzero else 0, K.ptr(ids), out.num_units, out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
 
@@ -173,9 +187,8 @@ def mx_dequantize(rows: MxRows, *, dtype: torch.dtype = torch.float32, out: torc
                             (out.stride(0) < rows.batch and rows.num_units > 1)):
             raise ValueError("mx_dequantize: out's samples must be adjacent and its rows must not overlap")
     ld = max(out.stride(0), rows.batch)
-    with _on(rows.device):
-        call("pxb_mx_dequantize", rows.num_units, rows.batch, rows.codes.data_ptr(), rows.scales.data_ptr(),
-             _lib.MX[rows.fmt], out.data_ptr(), _DT[out.dtype], ld, K._stream())
+    _launch(rows.device, "pxb_mx_dequantize", rows.num_units, rows.batch, rows.codes.data_ptr(), rows.scales.data_ptr(),
+            _lib.MX[rows.fmt], out.data_ptr(), _DT[out.dtype], ld)
     return out
 
 
@@ -195,10 +208,8 @@ def mx_unit_apply(rows: torch.Tensor, checkpoint: MxRows, activation, *, level: 
     _format(checkpoint.fmt, CHECKPOINT_FORMATS, "checkpoint format")
     _tensor(rows, torch.float32, (checkpoint.num_units, checkpoint.batch), "mx_unit_apply: rows", checkpoint.device)
     _masks(n, rows.device, level, roles, "mx_unit_apply")
-    with _on(rows.device):
-        call("pxb_mx_unit_apply", n, b, _lib.act_code(activation), rows.data_ptr(), K.ptr(level), target_level,
-             K.ptr(roles), _lib.MX[checkpoint.fmt], checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr(),
-             K._stream())
+    _launch(rows.device, "pxb_mx_unit_apply", n, b, _lib.act_code(activation), rows.data_ptr(), K.ptr(level), target_level,
+            K.ptr(roles), _lib.MX[checkpoint.fmt], checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr())
 
 
 def mx_unit_grad(acc: torch.Tensor, act: MxRows, activation, *, seed: torch.Tensor | None = None,
@@ -219,10 +230,8 @@ def mx_unit_grad(acc: torch.Tensor, act: MxRows, activation, *, seed: torch.Tens
         out = torch.zeros_like(acc) if level is not None or roles is not None else torch.empty_like(acc)
     else:
         _tensor(out, torch.float32, shape, "mx_unit_grad: out", act.device)
-    with _on(acc.device):
-        call("pxb_mx_unit_grad", n, b, _lib.act_code(activation), acc.data_ptr(), K.ptr(seed), act.codes.data_ptr(),
-             act.scales.data_ptr(), _lib.MX[act.fmt], K.ptr(level), target_level, K.ptr(roles), out.data_ptr(),
-             K._stream())
+    _launch(acc.device, "pxb_mx_unit_grad", n, b, _lib.act_code(activation), acc.data_ptr(), K.ptr(seed), act.codes.data_ptr(),
+            act.scales.data_ptr(), _lib.MX[act.fmt], K.ptr(level), target_level, K.ptr(roles), out.data_ptr())
     return out
 
 
@@ -246,10 +255,9 @@ def mx_edge_grad(bucket: K.Bucket, grad: torch.Tensor, act: MxRows, *, out: torc
         out = torch.empty(cap, dtype=torch.float32, device=act.device)
     else:
         _tensor(out, torch.float32, (cap,), "mx_edge_grad: out", act.device)
-    with _on(act.device):
-        call("pxb_mx_edge_grad", cap, K.ptr(bucket["from_id"]), K.ptr(bucket["to_id"]), K.ptr(bucket["dead"]),
-             grad.data_ptr(), act.codes.data_ptr(), act.scales.data_ptr(), _lib.MX[act.fmt], act.batch,
-             act.num_units, out.data_ptr(), None, None, None, None, None, K._stream())
+    _launch(act.device, "pxb_mx_edge_grad", cap, K.ptr(bucket["from_id"]), K.ptr(bucket["to_id"]), K.ptr(bucket["dead"]),
+            grad.data_ptr(), act.codes.data_ptr(), act.scales.data_ptr(), _lib.MX[act.fmt], act.batch,
+            act.num_units, out.data_ptr(), None, None, None, None, None)
     return out
 
 
@@ -261,11 +269,10 @@ def mx_update(bucket: K.Bucket, grad: torch.Tensor, act: MxRows, opt: _lib.Optim
     for name in ("weight", "opt/m", "opt/v", "opt/t"):
         if name == "weight" or name in bucket:
             _tensor(bucket[name], torch.float32, (cap,), f"mx_update: bucket column {name!r}", act.device)
-    with _on(act.device):
-        call("pxb_mx_edge_grad", cap, K.ptr(bucket["from_id"]), K.ptr(bucket["to_id"]), K.ptr(bucket["dead"]),
-             grad.data_ptr(), act.codes.data_ptr(), act.scales.data_ptr(), _lib.MX[act.fmt], act.batch,
-             act.num_units, None, K.ptr(bucket["weight"]), ctypes.byref(opt), K.ptr(bucket.get("opt/m")),
-             K.ptr(bucket.get("opt/v")), K.ptr(bucket.get("opt/t")), K._stream())
+    _launch(act.device, "pxb_mx_edge_grad", cap, K.ptr(bucket["from_id"]), K.ptr(bucket["to_id"]), K.ptr(bucket["dead"]),
+            grad.data_ptr(), act.codes.data_ptr(), act.scales.data_ptr(), _lib.MX[act.fmt], act.batch,
+            act.num_units, None, K.ptr(bucket["weight"]), ctypes.byref(opt), K.ptr(bucket.get("opt/m")),
+            K.ptr(bucket.get("opt/v")), K.ptr(bucket.get("opt/t")))
 
 
 @dataclasses.dataclass(frozen=True)
@@ -370,12 +377,11 @@ def mx_product(conns: MxConns, x: torch.Tensor | MxRows, *, activation: str = "i
     else:
         rows, _ = _rows_shape(out, "mx_product: out")
         _tensor(out, torch.float32, (rows, b), "mx_product: out", dev)
-    with _on(dev):
-        call("pxb_mx_product", ctypes.byref(conns._c), n, b, None if mx_in else x.data_ptr(),
-             x.codes.data_ptr() if mx_in else None, x.scales.data_ptr() if mx_in else None,
-             _lib.MX[x.fmt] if mx_in else _lib.MX["f32"], _lib.ACT[activation], rows,
-             None if mx_out else out.data_ptr(), out.codes.data_ptr() if mx_out else None,
-             out.scales.data_ptr() if mx_out else None, _lib.MX[out.fmt] if mx_out else _lib.MX["f32"], K._stream())
+    _launch(dev, "pxb_mx_product", ctypes.byref(conns._c), n, b, None if mx_in else x.data_ptr(),
+            x.codes.data_ptr() if mx_in else None, x.scales.data_ptr() if mx_in else None,
+            _lib.MX[x.fmt] if mx_in else _lib.MX["f32"], _lib.ACT[activation], rows,
+            None if mx_out else out.data_ptr(), out.codes.data_ptr() if mx_out else None,
+            out.scales.data_ptr() if mx_out else None, _lib.MX[out.fmt] if mx_out else _lib.MX["f32"])
     return out
 
 

@@ -50,7 +50,8 @@ __host__ __device__ inline int64_t mx_blocks(int64_t n) { return (n + kMxBlock -
 
 // The value of a scale byte.
 __device__ __forceinline__ float mx_scale_value(uint32_t s) {
-  return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23);
+  // the exponent field; 0 (2^-127, a subnormal) and 255 (not a number) set the same mantissa bit
+  return __uint_as_float((s << 23) | (((s + 1) & 0xfeu) == 0 ? 0x00400000u : 0u));
 }
 
 // The scale byte of a block whose largest magnitude has these bits.
@@ -174,6 +175,20 @@ __device__ __forceinline__ uint32_t mx_amax8(const float (&x)[8]) {
   for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
   return m;
 }
+
+// Division by a launch constant: n / d for n < 2^32 as a multiply-high
+// (round-up method; exact for every 32-bit n with a 33-bit magic number).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  explicit FastDiv(uint32_t div) : d(div), mul(0), shift(0) {
+    while ((uint64_t(1) << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    const uint64_t t = __umulhi(n, mul);
+    return static_cast<uint32_t>((t + n) >> shift);
+  }
+};
 
 // CTAs for a kernel whose CTAs step through `items`, `per_cta` at a time: one
 // full wave at most (a grid of 8 an SM where 6 fit would leave a second wave a

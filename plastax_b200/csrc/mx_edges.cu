@@ -265,55 +265,182 @@ struct Out {
   uint32_t rows;
   float *x;
   uint8_t *codes, *scales;
+  bool vec;  // float32 rows on 16-byte boundaries
 };
 
-template <int XF>
 struct Rows {
   const float *__restrict__ x;
   const uint8_t *__restrict__ codes;
   const uint8_t *__restrict__ scales;
   int32_t batch, nb;
-
-  // samples in the 16 bytes that a lane loads at once, and the lanes a row takes at most
-  static constexpr int kPiece = XF == PXB_MX_F32 ? 4 : XF == PXB_MX_E2M1 ? 32 : 16;
-  static constexpr int kMaxLanes = XF == PXB_MX_F32 ? 32 : 256 / kPiece;
+  uint32_t rows;
 };
 
-// One loaded piece of a source row and the factor of its values.
+// A launch's items: (destination, chunk of the batch), `wpd` warps of a CTA to
+// an item, 8 / wpd items a tile, a tile a cluster (of one CTA or more).
+struct Items {
+  uint32_t total, tiles;
+  FastDiv chunks;
+  int wpd;
+};
+
+struct Item {
+  int64_t e0, blk0;
+  int32_t blocks, tail;  // of 32 edges, the last with `tail`
+  int32_t chunk;
+};
+
+__device__ __forceinline__ Item load_item(const Conns &c, const Items &n, uint32_t item) {
+  const uint32_t i = n.chunks.div(item);
+  Item t;
+  t.chunk = static_cast<int32_t>(item - i * n.chunks.d);
+  t.e0 = max(int64_t(0), __ldg(c.offsets + i));
+  t.blk0 = c.fmt == PXB_MX_F32 ? 0 : max(int64_t(0), __ldg(c.block_offsets + i));
+  const int64_t edges = max(int64_t(0), min(c.num_edges, __ldg(c.offsets + i + 1)) - t.e0);
+  t.blocks = static_cast<int32_t>(min((edges + 31) >> 5, int64_t(0x7fffffff)));
+  t.tail = static_cast<int32_t>(edges - (static_cast<int64_t>(t.blocks) - 1) * 32);
+  return t;
+}
+
+// Lane's edge of block k: its source (-1 for none) and weight.
+__device__ __forceinline__ void load_edge(const Conns &c, const Item &it, int32_t k, int lane, uint32_t rows, int32_t &s,
+                                          float &w) {
+  s = -1;
+  w = 0.0f;
+  if (k < it.blocks - 1 || (k == it.blocks - 1 && lane < it.tail)) {
+    const int64_t e = it.e0 + static_cast<int64_t>(k) * 32 + lane;
+    const int32_t v = __ldg(c.src + e);
+    const float x = conn_weight(c, e, it.blk0 + k, lane);
+    if (static_cast<uint32_t>(v) < rows) s = v, w = x;
+  }
+}
+
+// One octet of an item's sums -> activation -> float32 or codes (every lane of
+// the warp calls; the four lanes of a block are neighbours).
+template <int CHUNK, typename Sum>
+__device__ __forceinline__ void finish_octet(const Conns &c, const Rows &r, int act_kind, const Out &out, const Items &n,
+                                             uint32_t item, int o, bool live, Sum sum) {
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  int32_t u = -1, b = 0;
+  if (live) {
+    const uint32_t i = n.chunks.div(item);
+    u = __ldg(c.units + i);
+    b = static_cast<int32_t>(item - i * n.chunks.d) * CHUNK + o;
+    sum(v);
+#pragma unroll
+    for (int z = 0; z < 8; ++z) v[z] = b + z < r.batch ? act_fn(act_kind, v[z]) : 0.0f;
+  }
+  const bool on = live && b < r.nb * kMxBlock && static_cast<uint32_t>(u) < out.rows;
+  if (out.fmt == PXB_MX_F32) {
+    float *dst = out.x + static_cast<int64_t>(u) * r.batch + b;
+    if (on && out.vec && b + 8 <= r.batch) {
+      reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else if (on) {
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (b + z < r.batch) dst[z] = v[z];
+    }
+  } else {
+    const int64_t at = static_cast<int64_t>(u) * r.nb * 4 + (b >> 3);
+    if (out.fmt == PXB_MX_E4M3) store_codes<PXB_MX_E4M3>(v, on, at, out.codes, out.scales);
+    else if (out.fmt == PXB_MX_E5M2) store_codes<PXB_MX_E5M2>(v, on, at, out.codes, out.scales);
+    else store_codes<PXB_MX_E2M1>(v, on, at, out.codes, out.scales);
+  }
+}
+
+// The sums of a tile's items lie in shared memory, one set a warp (`stride`
+// floats apart, CHUNK samples each). An item of one warp is finished by it;
+// else the CTA's first threads, of the cluster's first CTA, join an item's sets
+// in order and finish it.
+template <int CHUNK>
+__device__ __forceinline__ void finish_items(const Conns &c, const Rows &r, int act_kind, const Out &out, const Items &n,
+                                             uint32_t tile, int ranks, float *part, int stride) {
+  constexpr int kOctets = (CHUNK < kMxBlock ? kMxBlock : CHUNK) / 8;  // an item's octets: whole blocks
+  namespace cg = cooperative_groups;
+  const auto add = [](float(&v)[8], const float *q, int o) {
+#pragma unroll
+    for (int z = 0; z < 8; ++z)
+      if (CHUNK % 8 == 0 ? o < CHUNK : o + z < CHUNK) v[z] += q[o + z];
+  };
+  if (n.wpd == 1 && ranks == 1) {
+    __syncwarp();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t item = tile * 8 + warp;
+#pragma unroll
+    for (int t = 0; t < (kOctets + 31) / 32 * 32; t += 32) {
+      const int o = (t + lane) * 8;
+      finish_octet<CHUNK>(c, r, act_kind, out, n, item, o, item < n.total && t + lane < kOctets,
+                               [&](float(&v)[8]) { add(v, part + warp * stride, o); });
+    }
+    __syncwarp();
+    return;
+  }
+  const cg::cluster_group cluster = cg::this_cluster();
+  if (ranks > 1) cluster.sync();
+  else __syncthreads();
+  if (ranks == 1 || cluster.block_rank() == 0) {
+    const int per_cta = 8 / n.wpd;
+    // every warp steps through whole rounds, so that a block's four lanes meet in the shuffles
+    for (int t = threadIdx.x; t < ((per_cta * kOctets + 31) & ~31); t += 256) {
+      const int j = t / kOctets, o = (t - j * kOctets) * 8;
+      const uint32_t item = tile * per_cta + j;
+      finish_octet<CHUNK>(c, r, act_kind, out, n, item, o, j < per_cta && item < n.total, [&](float(&v)[8]) {
+        for (int k = 0; k < ranks; ++k) {
+          const float *q = ranks > 1 ? cluster.map_shared_rank(part, k) : part;
+          for (int m = 0; m < n.wpd; ++m) add(v, q + (j * n.wpd + m) * stride, o);
+        }
+      });
+    }
+  }
+  if (ranks > 1) cluster.sync();
+  else __syncthreads();
+}
+
+// 16 bytes of a source row (a piece: a block of 32 samples in e2m1, 16 samples
+// in 8 bits, 4 in float32) and the factor of its values.
+template <int XF>
 struct Piece {
+  static constexpr int kSamples = XF == PXB_MX_F32 ? 4 : XF == PXB_MX_E2M1 ? 32 : 16;
+  static constexpr int kMaxLanes = XF == PXB_MX_F32 ? 32 : 256 / kSamples;  // lanes a row takes at most
   uint4 v;
   float w;
 };
 
-template <int XF, bool VEC>
-__device__ __forceinline__ Piece load_piece(const Rows<XF> &r, int32_t src, float w, int32_t piece, bool on) {
-  Piece p{make_uint4(0, 0, 0, 0), 0.0f};
-  if (!on || src < 0) return p;
+// Offsets of rows in bytes; one past every row where the edge has no source.
+template <typename O>
+constexpr O kNoRow = ~O(0);
+
+template <int XF, bool VEC, typename O>
+__device__ __forceinline__ Piece<XF> load_piece(const Rows &r, O row, float w, int32_t piece, bool on) {
+  Piece<XF> p;
+  p.v = make_uint4(0, 0, 0, 0);
+  p.w = 0.0f;
+  if (!on || row == kNoRow<O>) return p;
   if constexpr (XF == PXB_MX_F32) {
-    const int32_t b = piece * 4;
-    const float *x = r.x + static_cast<int64_t>(src) * r.batch + b;
+    const float *x = reinterpret_cast<const float *>(reinterpret_cast<const char *>(r.x) + row) + piece * 4;
     p.w = w;
     if (VEC) {
       p.v = __ldg(reinterpret_cast<const uint4 *>(x));
     } else {
       const uint32_t *u = reinterpret_cast<const uint32_t *>(x);
+      const int32_t left = r.batch - piece * 4;
       p.v.x = __ldg(u);
-      if (b + 1 < r.batch) p.v.y = __ldg(u + 1);
-      if (b + 2 < r.batch) p.v.z = __ldg(u + 2);
-      if (b + 3 < r.batch) p.v.w = __ldg(u + 3);
+      if (left > 1) p.v.y = __ldg(u + 1);
+      if (left > 2) p.v.z = __ldg(u + 2);
+      if (left > 3) p.v.w = __ldg(u + 3);
     }
   } else {
-    constexpr int kPerBlock = kMxBlock / Rows<XF>::kPiece;
-    const int64_t row = static_cast<int64_t>(src) * r.nb;
-    p.v = __ldg(reinterpret_cast<const uint4 *>(r.codes) + row * kPerBlock + piece);
-    p.w = __fmul_rn(w, mx_scale_value(__ldg(r.scales + row + piece / kPerBlock)));
+    constexpr int kShift = XF == PXB_MX_E2M1 ? 4 : 5;  // a block's bytes of codes
+    p.v = __ldg(reinterpret_cast<const uint4 *>(r.codes + row) + piece);
+    p.w = __fmul_rn(w, mx_scale_value(__ldg(r.scales + (row >> kShift) + (piece >> (kShift - 4)))));
   }
   return p;
 }
 
 // acc += w * values, two at a time.
 template <int XF>
-__device__ __forceinline__ void add_piece(const Piece &p, float2 (&acc)[Rows<XF>::kPiece / 2]) {
+__device__ __forceinline__ void add_piece(const Piece<XF> &p, float2 (&acc)[Piece<XF>::kSamples / 2]) {
   const uint32_t v[4] = {p.v.x, p.v.y, p.v.z, p.v.w};
   const float2 w = make_float2(p.w, p.w);
   if constexpr (XF == PXB_MX_F32) {
@@ -331,57 +458,52 @@ __device__ __forceinline__ void add_piece(const Piece &p, float2 (&acc)[Rows<XF>
   }
 }
 
-// The edges of a destination are cut into blocks of 32 (the weights' blocks).
-// A warp takes a block: lane j holds edge j's source and weight. A source row
-// is LANES pieces of 16 bytes (a whole block of 32 samples in e2m1, 16 samples
-// in 8 bits, 4 in float32), so 32 / LANES edges are read side by side, each
-// load instruction full, up to four in flight a lane. `wpd` warps of a block
-// and, where destinations are few and long, the CTAs of a cluster share a
-// destination's blocks; their sums join in shared memory (a peer CTA's through
-// the cluster) in a fixed order, and one octet a thread then takes the
-// activation and leaves as float32 or as codes.
-template <int XF, int LANES, bool VEC>
-__global__ void __launch_bounds__(256) mx_product_kernel(Conns c, uint32_t num_src, Rows<XF> r, int act_kind, Out out,
-                                                         int32_t chunks, int wpd) {
-  constexpr int A = Rows<XF>::kPiece, kGroups = 32 / LANES, kChunk = LANES * A;
-  constexpr int kOctets = (kChunk < kMxBlock ? kMxBlock : kChunk) / 8;  // an item's octets: whole blocks
-  constexpr int kDepth = LANES < 4 ? LANES : 4;
-  __shared__ float part[8][kChunk];
+// A warp takes a block of 32 edges of an item: lane j holds edge j's row and
+// weight, and fetches the next block's while this one's rows come. A row is
+// LANES pieces, so 32 / LANES edges are read side by side, each load
+// instruction full, two in flight a lane. The loop waits on L2 and issues about
+// three instructions a pair of samples (two conversions and a paired FMA, on
+// two pipes), so warps count for more than loads a warp: 64 registers, 32 warps
+// an SM.
+template <int XF, int LANES, bool VEC, bool WIDE>
+__global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int act_kind, Out out, Items n) {
+  using O = typename Offset<WIDE>::type;
+  constexpr int A = Piece<XF>::kSamples, kGroups = 32 / LANES, kChunk = LANES * A, kDepth = LANES < 2 ? 1 : 2;
+  __shared__ __align__(16) float part[8][kChunk];
   namespace cg = cooperative_groups;
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES, grp = lane / LANES;
-  const int team = warp / wpd, member = warp % wpd, per_cta = 8 / wpd;
+  const int team = warp / n.wpd, member = warp % n.wpd, per_cta = 8 / n.wpd;
   const int32_t pieces = XF == PXB_MX_F32 ? (r.batch + 3) / 4 : r.nb * (kMxBlock / A);
-  const int64_t total = static_cast<int64_t>(c.num_dst) * chunks, tiles = (total + per_cta - 1) / per_cta;
-  for (int64_t tile = blockIdx.x / ranks; tile < tiles; tile += gridDim.x / ranks) {
-    const int64_t item = tile * per_cta + team;
+  const O row_bytes = XF == PXB_MX_F32 ? static_cast<O>(r.batch) * 4 : static_cast<O>(pieces) * 16;
+  const int32_t step = n.wpd * ranks;
+  for (uint32_t tile = blockIdx.x / ranks; tile < n.tiles; tile += gridDim.x / ranks) {
+    const uint32_t item = tile * per_cta + team;
     float2 acc[A / 2];
 #pragma unroll
     for (int q = 0; q < A / 2; ++q) acc[q] = make_float2(0.0f, 0.0f);
-    if (item < total) {
-      const int32_t i = static_cast<int32_t>(item / chunks);
-      const int32_t piece = static_cast<int32_t>(item - static_cast<int64_t>(i) * chunks) * LANES + sub;
+    if (item < n.total) {
+      const Item it = load_item(c, n, item);
+      const int32_t piece = it.chunk * LANES + sub;
       const bool on = piece < pieces;
-      const int64_t e0 = max(int64_t(0), __ldg(c.offsets + i)), e1 = min(c.num_edges, __ldg(c.offsets + i + 1));
-      const int64_t blk0 = c.fmt == PXB_MX_F32 ? 0 : max(int64_t(0), __ldg(c.block_offsets + i));
-      for (int64_t k = member + rank * wpd; e0 + k * 32 < e1; k += wpd * ranks) {
-        const int64_t e = e0 + k * 32 + lane;
-        int32_t s = -1;
-        float w = 0.0f;
-        if (e < e1) {
-          s = __ldg(c.src + e);
-          if (static_cast<uint32_t>(s) >= num_src) s = -1;
-          w = conn_weight(c, e, blk0 + k, lane);
-        }
-        const int cnt = static_cast<int>(min(int64_t(32), e1 - e0 - k * 32));
+      int32_t k = member + rank * n.wpd, next;
+      float next_w;
+      load_edge(c, it, k, lane, r.rows, next, next_w);
+#pragma unroll 1
+      for (; k < it.blocks; k += step) {
+        const O row = next < 0 ? kNoRow<O> : static_cast<O>(next) * row_bytes;
+        const float w = next_w;
+        load_edge(c, it, k + step, lane, r.rows, next, next_w);
+        const int cnt = k == it.blocks - 1 ? it.tail : 32;
 #pragma unroll 1
         for (int j = 0; j < cnt; j += kGroups * kDepth) {
-          Piece p[kDepth];
+          Piece<XF> p[kDepth];
 #pragma unroll
           for (int d = 0; d < kDepth; ++d) {
             const int at = j + d * kGroups + grp;
-            p[d] = load_piece<XF, VEC>(r, __shfl_sync(0xffffffffu, s, at), __shfl_sync(0xffffffffu, w, at), piece, on);
+            p[d] = load_piece<XF, VEC, O>(r, LANES == 1 ? row : __shfl_sync(0xffffffffu, row, at),
+                                          LANES == 1 ? w : __shfl_sync(0xffffffffu, w, at), piece, on);
           }
 #pragma unroll
           for (int d = 0; d < kDepth; ++d) add_piece<XF>(p[d], acc);
@@ -395,82 +517,48 @@ __global__ void __launch_bounds__(256) mx_product_kernel(Conns c, uint32_t num_s
     int base = sub * A;
     constexpr int kHeld = A > kGroups ? A / kGroups : 1;
 #pragma unroll
-    for (int off = 16, n = A; off >= LANES; off >>= 1) {
-      if (n > 1) {
-        n >>= 1;
+    for (int off = 16, left = A; off >= LANES; off >>= 1) {
+      if (left > 1) {
+        left >>= 1;
         const bool upper = (lane & off) != 0;
 #pragma unroll
-        for (int q = 0; q < n; ++q) {
-          const float send = upper ? f[q] : f[q + n], keep = upper ? f[q + n] : f[q];
+        for (int q = 0; q < left; ++q) {
+          const float send = upper ? f[q] : f[q + left], keep = upper ? f[q + left] : f[q];
           f[q] = keep + __shfl_xor_sync(0xffffffffu, send, off);
         }
-        base += upper ? n : 0;
+        base += upper ? left : 0;
       } else {
         f[0] += __shfl_xor_sync(0xffffffffu, f[0], off);
       }
     }
 #pragma unroll
     for (int q = 0; q < kHeld; ++q) part[warp][base + q] = f[q];
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-    if (rank == 0) {
-      // every warp steps through whole rounds, so that a block's four lanes meet in the shuffles
-      for (int t = threadIdx.x; t < ((per_cta * kOctets + 31) & ~31); t += 256) {
-        const int j = t / kOctets, o = (t - j * kOctets) * 8;
-        const int64_t it = tile * per_cta + j;
-        const bool live = j < per_cta && it < total;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        int32_t u = -1, b = 0;
-        if (live) {
-          const int32_t i = static_cast<int32_t>(it / chunks);
-          u = __ldg(c.units + i);
-          b = static_cast<int32_t>(it - static_cast<int64_t>(i) * chunks) * kChunk + o;
-          for (int k = 0; k < ranks; ++k) {
-            const float *q = ranks > 1 ? cluster.map_shared_rank(&part[0][0], k) : &part[0][0];
-            for (int m = 0; m < wpd; ++m)
-#pragma unroll
-              for (int z = 0; z < 8; ++z)
-                if (o + z < kChunk) v[z] += q[(j * wpd + m) * kChunk + o + z];
-          }
-#pragma unroll
-          for (int z = 0; z < 8; ++z) v[z] = b + z < r.batch ? act_fn(act_kind, v[z]) : 0.0f;
-        }
-        const bool on = live && b < r.nb * kMxBlock && static_cast<uint32_t>(u) < out.rows;
-        if (out.fmt == PXB_MX_F32) {
-          float *dst = out.x + static_cast<int64_t>(u) * r.batch + b;
-          if (on && VEC && b + 8 <= r.batch) {
-            reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else if (on) {
-#pragma unroll
-            for (int z = 0; z < 8; ++z)
-              if (b + z < r.batch) dst[z] = v[z];
-          }
-        } else {
-          const int64_t at = static_cast<int64_t>(u) * r.nb * 4 + (b >> 3);
-          if (out.fmt == PXB_MX_E4M3) store_codes<PXB_MX_E4M3>(v, on, at, out.codes, out.scales);
-          else if (out.fmt == PXB_MX_E5M2) store_codes<PXB_MX_E5M2>(v, on, at, out.codes, out.scales);
-          else store_codes<PXB_MX_E2M1>(v, on, at, out.codes, out.scales);
-        }
-      }
-    }
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
+    finish_items<kChunk>(c, r, act_kind, out, n, tile, ranks, &part[0][0], kChunk);
   }
 }
 
-template <int XF, int LANES, bool VEC>
-static int launch_product_as(const Conns &c, int32_t num_src, const Rows<XF> &r, int act, const Out &out, int32_t chunks,
-                             cudaStream_t st) {
-  const int64_t items = static_cast<int64_t>(c.num_dst) * chunks, mean = c.num_edges / c.num_dst;
+// How many warps share a destination (`wpd`, up to a CTA's eight) and, past
+// that, CTAs: until every SM has 32 warps' worth or a warp has one block of 32
+// edges left.
+static void split_items(int64_t items, int64_t mean, int *wpd, int *ranks) {
   const int64_t warps = static_cast<int64_t>(sm_count()) * 32;
-  int wpd = 1, ranks = 1;
-  while (wpd < 8 && items * wpd < warps && mean > 32 * wpd) wpd *= 2;
-  if (wpd == 8)
-    while (ranks < 8 && items * 8 * ranks < warps && mean > 32 * 8 * ranks) ranks *= 2;
-  const int64_t tiles = (items * wpd + 7) / 8, most = static_cast<int64_t>(sm_count()) * 8;
+  *wpd = *ranks = 1;
+  while (*wpd < 8 && items * *wpd < warps && mean > 32 * *wpd) *wpd *= 2;
+  if (*wpd == 8)
+    while (*ranks < 8 && items * 8 * *ranks < warps && mean > 32 * 8 * *ranks) *ranks *= 2;
+}
+
+template <auto KERNEL>
+static int launch_items(const Conns &c, const Rows &r, int act, const Out &out, int32_t chunks, cudaStream_t st) {
+  const int64_t items = static_cast<int64_t>(c.num_dst) * chunks;
+  PXB_REQUIRE(items < (int64_t(1) << 32) - 8, "pxb_mx_product: %lld destinations and chunks are past 2^32",
+              static_cast<long long>(items));
+  int wpd, ranks;
+  split_items(items, c.num_edges / c.num_dst, &wpd, &ranks);
+  const int64_t tiles = (items * wpd + 7) / 8;
+  const Items n{static_cast<uint32_t>(items), static_cast<uint32_t>(tiles), FastDiv(static_cast<uint32_t>(chunks)), wpd};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((tiles < most ? tiles : most) * ranks));
+  cfg.gridDim = dim3(static_cast<unsigned>(mx_grid<KERNEL>(tiles, 1, 256) * ranks));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -478,22 +566,27 @@ static int launch_product_as(const Conns &c, int32_t num_src, const Rows<XF> &r,
   attr.val.clusterDim.x = ranks;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  PXB_CUDA(cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, LANES, VEC>, c, static_cast<uint32_t>(num_src), r, act, out,
-                              chunks, wpd));
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  PXB_CUDA(cudaLaunchKernelEx(&cfg, KERNEL, c, r, act, out, n));
   return PXB_OK;
 }
 
 template <int XF, int LANES>
-static int launch_product(const Conns &c, int32_t num_src, const Rows<XF> &r, int act, const Out &out, bool vec,
-                          cudaStream_t st) {
-  const int32_t pieces = XF == PXB_MX_F32 ? (r.batch + 3) / 4 : r.nb * (kMxBlock / Rows<XF>::kPiece);
-  if constexpr (LANES < Rows<XF>::kMaxLanes) {
-    if (pieces > LANES) return launch_product<XF, LANES * 2>(c, num_src, r, act, out, vec, st);
+static int launch_product(const Conns &c, const Rows &r, int act, const Out &out, bool vec, cudaStream_t st) {
+  const int32_t pieces = XF == PXB_MX_F32 ? (r.batch + 3) / 4 : r.nb * (kMxBlock / Piece<XF>::kSamples);
+  if constexpr (LANES < Piece<XF>::kMaxLanes) {
+    if (pieces > LANES) return launch_product<XF, LANES * 2>(c, r, act, out, vec, st);
   }
   const int32_t chunks = (pieces + LANES - 1) / LANES;
-  if (vec) return launch_product_as<XF, LANES, true>(c, num_src, r, act, out, chunks, st);
-  return launch_product_as<XF, LANES, false>(c, num_src, r, act, out, chunks, st);
+  const int64_t row_bytes = XF == PXB_MX_F32 ? int64_t(r.batch) * 4 : int64_t(pieces) * 16;
+  const bool wide = r.rows * row_bytes >= (int64_t(1) << 32);
+  if constexpr (XF == PXB_MX_F32) {
+    if (!vec)
+      return wide ? launch_items<mx_product_kernel<XF, LANES, false, true>>(c, r, act, out, chunks, st)
+                  : launch_items<mx_product_kernel<XF, LANES, false, false>>(c, r, act, out, chunks, st);
+  }
+  return wide ? launch_items<mx_product_kernel<XF, LANES, true, true>>(c, r, act, out, chunks, st)
+              : launch_items<mx_product_kernel<XF, LANES, true, false>>(c, r, act, out, chunks, st);
 }
 
 template <int FMT, bool VEC, bool WIDE>
@@ -585,14 +678,12 @@ extern "C" int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src, int32_
   const Conns c{conns->num_dst, conns->fmt, conns->num_edges, conns->num_blocks, conns->units, conns->offsets, conns->src,
                 conns->weight, conns->block_offsets, conns->codes, conns->scales};
   const int32_t nb = static_cast<int32_t>(mx_blocks(batch));
-  const bool vec = batch % 4 == 0 && aligned16(x) && aligned16(out);
   cudaStream_t st = as_stream(stream);
-  const Out o{out_fmt, static_cast<uint32_t>(num_out), out, out_codes, out_scales};
-#define PXB_MXD(XF) \
-  launch_product<XF, kMxBlock / (XF == PXB_MX_F32 ? kMxBlock : Rows<XF>::kPiece)>(c, num_src, Rows<XF>{x, x_codes, x_scales, batch, nb}, act_kind, o, vec, st)
-  if (x_fmt == PXB_MX_F32) return PXB_MXD(PXB_MX_F32);
-  if (x_fmt == PXB_MX_E4M3) return PXB_MXD(PXB_MX_E4M3);
-  if (x_fmt == PXB_MX_E5M2) return PXB_MXD(PXB_MX_E5M2);
-  return PXB_MXD(PXB_MX_E2M1);
-#undef PXB_MXD
+  const bool whole = batch % 4 == 0;
+  const Out o{out_fmt, static_cast<uint32_t>(num_out), out, out_codes, out_scales, whole && aligned16(out)};
+  const Rows r{x, x_codes, x_scales, batch, nb, static_cast<uint32_t>(num_src)};
+  if (x_fmt == PXB_MX_F32) return launch_product<PXB_MX_F32, 1>(c, r, act_kind, o, whole && aligned16(x), st);
+  if (x_fmt == PXB_MX_E4M3) return launch_product<PXB_MX_E4M3, 2>(c, r, act_kind, o, true, st);
+  if (x_fmt == PXB_MX_E5M2) return launch_product<PXB_MX_E5M2, 2>(c, r, act_kind, o, true, st);
+  return launch_product<PXB_MX_E2M1, 1>(c, r, act_kind, o, true, st);
 }

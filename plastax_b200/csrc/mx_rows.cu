@@ -12,20 +12,6 @@
 
 namespace pxb {
 
-// Division by a launch constant: n / d for n < 2^32 as a multiply-high
-// (round-up method; exact for every 32-bit n with a 33-bit magic number).
-struct FastDiv {
-  uint32_t d, mul, shift;
-  explicit FastDiv(uint32_t div) : d(div), mul(0), shift(0) {
-    while ((uint64_t(1) << shift) < d) ++shift;
-    mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const {
-    const uint64_t t = __umulhi(n, mul);
-    return static_cast<uint32_t>((t + n) >> shift);
-  }
-};
-
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
   return static_cast<float>(v);

@@ -22,6 +22,15 @@ namespace pxb {
 
 constexpr int kMxBlock = 32;
 
+// A value's bits as another type of its size.
+template <typename To, typename From>
+__device__ __forceinline__ To same_bits(const From &v) {
+  static_assert(sizeof(To) == sizeof(From), "sizes differ");
+  To t;
+  memcpy(&t, &v, sizeof(To));
+  return t;
+}
+
 template <int FMT>
 struct MxFormat;
 template <>
@@ -78,30 +87,33 @@ __device__ __forceinline__ uint64_t mx_encode8(const float (&x)[8], uint32_t sca
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(x[i], inv);
+  // Each pair leaves the assembly as a whole register and the pairs are joined
+  // here: packed inside it (mov.b32 {a, b}), two pairs of equal values that the
+  // compiler had merged came out with an undefined upper half.
   uint32_t lo, hi = 0;
   if constexpr (FMT == PXB_MX_E2M1) {
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\tcvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
-        : "=r"(lo) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}"
+          : "=r"(c[i]) : "f"(y[2 * i]), "f"(y[2 * i + 1]));
+    lo = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     if (keep) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (x[i] != 0.0f && (lo & (0x7u << (4 * i))) == 0) lo |= 0x1u << (4 * i);
     }
   } else {
-#define PXB_MX_ENCODE4(KIND, OUT, AT)                                                                            \
-  asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite." KIND "x2.f32 a, %2, %1;\n\tcvt.rn.satfinite." KIND         \
-      "x2.f32 b, %4, %3;\n\tmov.b32 %0, {a, b};\n\t}"                                                          \
-      : "=r"(OUT) : "f"(y[AT]), "f"(y[AT + 1]), "f"(y[AT + 2]), "f"(y[AT + 3]))
-    if constexpr (FMT == PXB_MX_E4M3) {
-      PXB_MX_ENCODE4("e4m3", lo, 0);
-      PXB_MX_ENCODE4("e4m3", hi, 4);
-    } else {
-      PXB_MX_ENCODE4("e5m2", lo, 0);
-      PXB_MX_ENCODE4("e5m2", hi, 4);
+    uint16_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (FMT == PXB_MX_E4M3)
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(c[i]) : "f"(y[2 * i]), "f"(y[2 * i + 1]));
+      else
+        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %2, %1;" : "=h"(c[i]) : "f"(y[2 * i]), "f"(y[2 * i + 1]));
     }
-#undef PXB_MX_ENCODE4
+    lo = __byte_perm(c[0], c[1], 0x5410);
+    hi = __byte_perm(c[2], c[3], 0x5410);
     if (keep) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -114,10 +126,11 @@ __device__ __forceinline__ uint64_t mx_encode8(const float (&x)[8], uint32_t sca
 }
 
 // Four bytes of codes (4 in 8 bits, 8 in e2m1) -> pairs of values before the
-// scale. Every element is a half; the conversions are the hardware's.
+// scale. Every element is a half; the conversions are the hardware's. For words
+// loaded whole (mx_decode2 takes parts of one).
 template <int FMT>
 __device__ __forceinline__ void mx_decode_word(uint32_t c, __half2 (&h)[32 / (2 * MxFormat<FMT>::bits)]) {
-  uint32_t *r = reinterpret_cast<uint32_t *>(h);
+  uint32_t r[32 / (2 * MxFormat<FMT>::bits)];
   if constexpr (FMT == PXB_MX_E2M1)
     asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t"
         "cvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
@@ -128,14 +141,17 @@ __device__ __forceinline__ void mx_decode_word(uint32_t c, __half2 (&h)[32 / (2 
   else
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e5m2x2 %0, a;\n\t"
         "cvt.rn.f16x2.e5m2x2 %1, b;\n\t}" : "=r"(r[0]), "=r"(r[1]) : "r"(c));
+#pragma unroll
+  for (int i = 0; i < 32 / (2 * MxFormat<FMT>::bits); ++i) h[i] = same_bits<__half2>(r[i]);
 }
 
-// The value of one code.
+// The two values of e2m1's byte, or of two bytes of the others, in c's low bits.
 template <int FMT>
-__device__ __forceinline__ float mx_decode1(uint32_t c) {
-  __half2 h[32 / (2 * MxFormat<FMT>::bits)];
-  mx_decode_word<FMT>(c, h);
-  return __low2float(h[0]);
+__device__ __forceinline__ float2 mx_decode2(uint32_t c) {
+  __half2_raw h;
+  if constexpr (FMT == PXB_MX_E2M1) h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(c), __NV_E2M1);
+  else h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c), FMT == PXB_MX_E4M3 ? __NV_E4M3 : __NV_E5M2);
+  return __half22float2(static_cast<__half2>(h));
 }
 
 // Eight codes -> eight values before the scale.

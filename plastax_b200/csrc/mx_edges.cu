@@ -83,12 +83,11 @@ __device__ __forceinline__ void load_acts(const EdgeGrad &k, int32_t f, int32_t 
 }
 
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
-  float2 d;
+  unsigned long long d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<unsigned long long &>(d))
-      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
-        "l"(reinterpret_cast<unsigned long long &>(c)));
-  return d;
+      : "=l"(d) : "l"(same_bits<unsigned long long>(a)), "l"(same_bits<unsigned long long>(b)),
+        "l"(same_bits<unsigned long long>(c)));
+  return same_bits<float2>(d);
 }
 
 // One slice of slot_sums: the group's eight slots' products into p. UNIFORM:
@@ -236,10 +235,10 @@ __device__ __forceinline__ float conn_weight(const Conns &c, int64_t edge, int64
   const float s = mx_scale_value(__ldg(c.scales + blk));
   float v;
   if (c.fmt == PXB_MX_E2M1) {
-    v = mx_decode1<PXB_MX_E2M1>(__ldg(c.codes + blk * 16 + (at >> 1)) >> (4 * (at & 1)));
+    v = mx_decode2<PXB_MX_E2M1>((__ldg(c.codes + blk * 16 + (at >> 1)) >> (4 * (at & 1))) & 0xfu).x;
   } else {
     const uint32_t code = __ldg(c.codes + blk * 32 + at);
-    v = c.fmt == PXB_MX_E4M3 ? mx_decode1<PXB_MX_E4M3>(code) : mx_decode1<PXB_MX_E5M2>(code);
+    v = c.fmt == PXB_MX_E4M3 ? mx_decode2<PXB_MX_E4M3>(code).x : mx_decode2<PXB_MX_E5M2>(code).x;
   }
   return __fmul_rn(v, s);
 }
@@ -487,7 +486,23 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
       const Item it = load_item(c, n, item);
       const int32_t piece = it.chunk * LANES + sub;
       const bool on = piece < pieces;
-      int32_t k = member + rank * n.wpd, next;
+      int32_t k = member + rank * n.wpd;
+      if constexpr (LANES == 1) {  // four blocks at once: a lane's edge has one piece
+#pragma unroll 1
+        for (; k < it.blocks; k += 4 * step) {
+          int32_t s[4];
+          float w[4];
+          Piece<XF> p[4];
+#pragma unroll
+          for (int d = 0; d < 4; ++d) load_edge(c, it, k + d * step, lane, r.rows, s[d], w[d]);
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            p[d] = load_piece<XF, VEC, O>(r, s[d] < 0 ? kNoRow<O> : static_cast<O>(s[d]) * row_bytes, w[d], piece, on);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) add_piece<XF>(p[d], acc);
+        }
+      }
+      int32_t next;
       float next_w;
       load_edge(c, it, k, lane, r.rows, next, next_w);
 #pragma unroll 1
@@ -502,8 +517,7 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
 #pragma unroll
           for (int d = 0; d < kDepth; ++d) {
             const int at = j + d * kGroups + grp;
-            p[d] = load_piece<XF, VEC, O>(r, LANES == 1 ? row : __shfl_sync(0xffffffffu, row, at),
-                                          LANES == 1 ? w : __shfl_sync(0xffffffffu, w, at), piece, on);
+            p[d] = load_piece<XF, VEC, O>(r, __shfl_sync(0xffffffffu, row, at), __shfl_sync(0xffffffffu, w, at), piece, on);
           }
 #pragma unroll
           for (int d = 0; d < kDepth; ++d) add_piece<XF>(p[d], acc);
@@ -534,6 +548,92 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
 #pragma unroll
     for (int q = 0; q < kHeld; ++q) part[warp][base + q] = f[q];
     finish_items<kChunk>(c, r, act_kind, out, n, tile, ranks, &part[0][0], kChunk);
+  }
+}
+
+// Up to four samples of float32 rows and many short destinations: eight lanes a
+// destination, four consecutive edges of a weight block each (their codes are
+// one load, their scale one), so a warp works on four destinations and the
+// set-up and the ending of each cost a quarter of a warp's. One sample of 32,768
+// destinations of 64 in-edges: 27 us with a warp each, 10 with eight lanes.
+__global__ void __launch_bounds__(256) mx_product_short_kernel(Conns c, Rows r, int act_kind, Out out) {
+  const int sub = threadIdx.x & 7;
+  const int64_t teams = static_cast<int64_t>(gridDim.x) * 32;
+  // whole warps step together (the shuffles below take every lane)
+  for (int64_t i0 = (blockIdx.x * int64_t(256) + threadIdx.x) / 32 * 4; i0 < c.num_dst; i0 += teams) {
+    const int64_t i = i0 + ((threadIdx.x & 31) >> 3);
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i < c.num_dst) {
+      const int64_t e0 = max(int64_t(0), __ldg(c.offsets + i)), e1 = min(c.num_edges, __ldg(c.offsets + i + 1));
+      int64_t blk = c.fmt == PXB_MX_F32 ? 0 : max(int64_t(0), __ldg(c.block_offsets + i));
+      for (int64_t e = e0 + sub * 4; e < e1; e += 32, ++blk) {
+        const int cnt = static_cast<int>(min(int64_t(4), e1 - e));
+        int32_t s[4];
+        float w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] = q < cnt ? __ldg(c.src + e + q) : -1;
+        if (c.fmt == PXB_MX_F32) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q < cnt) w[q] = __ldg(c.weight + e + q);
+        } else if (blk < c.num_blocks) {
+          const float scale = mx_scale_value(__ldg(c.scales + blk));
+          float2 lo, hi;
+          if (c.fmt == PXB_MX_E2M1) {
+            const uint32_t code = __ldg(reinterpret_cast<const uint16_t *>(c.codes + blk * 16) + sub);
+            lo = mx_decode2<PXB_MX_E2M1>(code & 0xffu), hi = mx_decode2<PXB_MX_E2M1>(code >> 8);
+          } else {
+            const uint32_t code = __ldg(reinterpret_cast<const uint32_t *>(c.codes + blk * 32) + sub);
+            if (c.fmt == PXB_MX_E4M3) lo = mx_decode2<PXB_MX_E4M3>(code & 0xffffu), hi = mx_decode2<PXB_MX_E4M3>(code >> 16);
+            else lo = mx_decode2<PXB_MX_E5M2>(code & 0xffffu), hi = mx_decode2<PXB_MX_E5M2>(code >> 16);
+          }
+          w[0] = __fmul_rn(lo.x, scale), w[1] = __fmul_rn(lo.y, scale);
+          w[2] = __fmul_rn(hi.x, scale), w[3] = __fmul_rn(hi.y, scale);
+        }
+        float x[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const bool on = static_cast<uint32_t>(s[q]) < r.rows;
+          const float *p = r.x + static_cast<int64_t>(s[q]) * r.batch;
+          if (!on) w[q] = 0.0f;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) x[q][b] = on && b < r.batch ? __ldg(p + b) : 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) f[b] = fmaf(w[q], x[q][b], f[b]);
+      }
+    }
+#pragma unroll
+    for (int off = 1; off < 8; off <<= 1)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) f[b] += __shfl_xor_sync(0xffffffffu, f[b], off);
+    const int32_t u = i < c.num_dst ? __ldg(c.units + i) : -1;
+    if (static_cast<uint32_t>(u) >= out.rows) continue;
+    if (out.fmt == PXB_MX_F32) {
+      const float v = sub == 0 ? f[0] : sub == 1 ? f[1] : sub == 2 ? f[2] : f[3];
+      if (sub < r.batch) out.x[static_cast<int64_t>(u) * r.batch + sub] = act_fn(act_kind, v);
+    } else if (sub < 4) {  // the block's octets, all but the first without samples
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < 4; ++b) v[b] = b < r.batch ? act_fn(act_kind, f[b]) : 0.0f;
+      const uint32_t m = mx_amax8(v);
+      if (sub > 0) v[0] = v[1] = v[2] = v[3] = 0.0f;
+      const int64_t at = static_cast<int64_t>(u) * 4 + sub;
+      uint32_t sb;
+      if (out.fmt == PXB_MX_E2M1) {
+        sb = mx_scale_byte<PXB_MX_E2M1>(m);
+        mx_store8<PXB_MX_E2M1>(out.codes, at, mx_encode8<PXB_MX_E2M1>(v, sb, false));
+      } else if (out.fmt == PXB_MX_E4M3) {
+        sb = mx_scale_byte<PXB_MX_E4M3>(m);
+        mx_store8<PXB_MX_E4M3>(out.codes, at, mx_encode8<PXB_MX_E4M3>(v, sb, false));
+      } else {
+        sb = mx_scale_byte<PXB_MX_E5M2>(m);
+        mx_store8<PXB_MX_E5M2>(out.codes, at, mx_encode8<PXB_MX_E5M2>(v, sb, false));
+      }
+      if (sub == 0) out.scales[u] = static_cast<uint8_t>(sb);
+    }
   }
 }
 
@@ -573,6 +673,14 @@ static int launch_items(const Conns &c, const Rows &r, int act, const Out &out, 
 
 template <int XF, int LANES>
 static int launch_product(const Conns &c, const Rows &r, int act, const Out &out, bool vec, cudaStream_t st) {
+  if constexpr (XF == PXB_MX_F32 && LANES == 1) {
+    // four short destinations a warp, as soon as that fills the SMs half
+    if (r.batch <= 4 && c.num_dst >= sm_count() * 64 && c.num_edges / c.num_dst <= 512) {
+      mx_product_short_kernel<<<mx_grid<mx_product_short_kernel>(c.num_dst, 32, 256), 256, 0, st>>>(c, r, act, out);
+      PXB_LAUNCHED("mx_product_short_kernel");
+      return PXB_OK;
+    }
+  }
   const int32_t pieces = XF == PXB_MX_F32 ? (r.batch + 3) / 4 : r.nb * (kMxBlock / Piece<XF>::kSamples);
   if constexpr (LANES < Piece<XF>::kMaxLanes) {
     if (pieces > LANES) return launch_product<XF, LANES * 2>(c, r, act, out, vec, st);
@@ -674,7 +782,8 @@ extern "C" int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src, int32_
                 "pxb_mx_product: x is NULL");
   }
   PXB_REQUIRE(out_fmt == PXB_MX_F32 ? out != nullptr : out_codes && out_scales, "pxb_mx_product: out is NULL");
-  PXB_REQUIRE(aligned16(x_codes) && aligned16(out_codes), "pxb_mx_product: codes must be 16-byte aligned");
+  PXB_REQUIRE(aligned16(x_codes) && aligned16(out_codes) && aligned16(conns->codes),
+              "pxb_mx_product: codes must be 16-byte aligned");
   const Conns c{conns->num_dst, conns->fmt, conns->num_edges, conns->num_blocks, conns->units, conns->offsets, conns->src,
                 conns->weight, conns->block_offsets, conns->codes, conns->scales};
   const int32_t nb = static_cast<int32_t>(mx_blocks(batch));

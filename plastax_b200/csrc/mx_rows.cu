@@ -92,6 +92,11 @@ struct Moves {
   }
 };
 
+template <typename T, int N>
+struct Pack {
+  T v[N];
+};
+
 // What a lane has read of its tile, before it is turned into its octet: the
 // words as they came, so that nothing waits between the loads.
 template <typename T, int LAYOUT>
@@ -156,9 +161,12 @@ __device__ __forceinline__ void settle(const Grid &g, const Octet &o, const Raw<
                                        float (&v)[8]) {
   if constexpr (LAYOUT == ALIGNED) {
     if (o.on && o.b + 8 <= g.batch) {
-      const T *h = reinterpret_cast<const T *>(r.v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_f32(h[i]);
+      for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q) {
+        const auto h = same_bits<Pack<T, 16 / sizeof(T)>>(r.v[q]);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) v[q * (16 / sizeof(T)) + i] = to_f32(h.v[i]);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = r.tail[i];
@@ -169,8 +177,8 @@ __device__ __forceinline__ void settle(const Grid &g, const Octet &o, const Raw<
 #pragma unroll
     for (int q = 0; q < Moves<LAYOUT>::kMoves; ++q) {
       if constexpr (LAYOUT == RUN2) {
-        const T *h = reinterpret_cast<const T *>(&r.v[q]);
-        reinterpret_cast<float2 *>(buf)[q * 32 + lane] = make_float2(to_f32(h[0]), to_f32(h[1]));
+        const auto h = same_bits<Pack<T, 2>>(r.v[q]);
+        reinterpret_cast<float2 *>(buf)[q * 32 + lane] = make_float2(to_f32(h.v[0]), to_f32(h.v[1]));
       } else {
         buf[q * 32 + lane] = to_f32(r.v[q]);
       }
@@ -208,11 +216,9 @@ __device__ __forceinline__ void put(const Grid &g, uint32_t tile, const Octet &o
           if (m.b(q) < end) p[q * 32] = from_f32<T>(buf[q * 32 + lane]);
         } else {
           const float2 two = reinterpret_cast<const float2 *>(buf)[q * 32 + lane];
-          uint32_t w;
-          T *h = reinterpret_cast<T *>(&w);
-          h[0] = from_f32<T>(two.x), h[1] = from_f32<T>(two.y);
-          if (m.b(q) < (end & ~1)) *reinterpret_cast<uint32_t *>(p + q * 64) = w;
-          if ((end & 1) && m.b(q) == end - 1) p[q * 64] = h[0];
+          const Pack<T, 2> h{from_f32<T>(two.x), from_f32<T>(two.y)};
+          if (m.b(q) < (end & ~1)) *reinterpret_cast<uint32_t *>(p + q * 64) = same_bits<uint32_t>(h);
+          if ((end & 1) && m.b(q) == end - 1) p[q * 64] = h.v[0];
         }
       }
     }
@@ -234,11 +240,10 @@ __device__ __forceinline__ void put(const Grid &g, uint32_t tile, const Octet &o
       if (fulls >> (lane | 1) & 1) *reinterpret_cast<float4 *>(odd ? p + 4 : p + 8) = odd ? make_float4(v[4], v[5], v[6], v[7]) : got;
       if (full) return;
     } else if (on && o.b + 8 <= g.batch) {
-      uint4 a;
-      T *h = reinterpret_cast<T *>(&a);
+      Pack<T, 8> h;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
-      *reinterpret_cast<uint4 *>(p) = a;
+      for (int i = 0; i < 8; ++i) h.v[i] = from_f32<T>(v[i]);
+      *reinterpret_cast<uint4 *>(p) = same_bits<uint4>(h);
       return;
     }
     if (on) {

@@ -36,8 +36,10 @@ from plastax_b200._lib import call
 BLOCK = 32
 FORMATS = ("e4m3", "e5m2", "e2m1")
 CHECKPOINT_FORMATS = ("e4m3", "e5m2")
+WEIGHT_FORMATS = (*FORMATS, "f32")
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MAX_BATCH = 1 << 24
+_U8 = torch.uint8
 
 
 def num_blocks(batch: int) -> int:
@@ -109,10 +111,16 @@ class MxRows:
     batch: int
 
     def __post_init__(self) -> None:
+        codes, scales = self.codes, self.scales
         _format(self.fmt)
         if not 0 <= self.batch <= _MAX_BATCH:
             raise ValueError(f"MxRows: batch must be in [0, {_MAX_BATCH}], got {self.batch}")
         nb = num_blocks(self.batch)
+        if isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype is _U8 and \
+                scales.dtype is _U8 and scales.dim() == 2 and scales.shape[1] == nb and \
+                codes.shape == (scales.shape[0], nb * block_bytes(self.fmt)) and codes.is_contiguous() and \
+                scales.is_contiguous() and codes.device == scales.device and codes.data_ptr() % 16 == 0:
+            return
         _tensor(self.scales, torch.uint8, None, "MxRows.scales")
         n = self.scales.shape[0] if self.scales.dim() == 2 else -1
         _tensor(self.scales, torch.uint8, (n, nb), "MxRows.scales")
@@ -158,7 +166,10 @@ def mx_quantize(x: torch.Tensor, fmt: str, *, keep_nonzero: bool = False, ids: t
     if out is None:
         if ids is not None:
             raise ValueError("mx_quantize: ids need out")
-        out = MxRows.empty(n, b, fmt, x.device)
+        out = object.__new__(MxRows)  # nothing to check in what is made here
+        nb = num_blocks(b)
+        out.__dict__.update(codes=x.new_empty((n, nb * block_bytes(fmt)), dtype=_U8),
+                            scales=x.new_empty((n, nb), dtype=_U8), fmt=fmt, batch=b)
     elif out.fmt != fmt or out.batch != b or out.device != x.device or (ids is None and out.num_units != n):
         raise ValueError(f"mx_quantize: out holds {out.num_units} x {out.batch} {out.fmt} rows on {out.device}, "
                          f"expected {n} x {b} {fmt} on {x.device}")
@@ -176,7 +187,7 @@ def mx_dequantize(rows: MxRows, *, dtype: torch.dtype = torch.float32, out: torc
     if out is None:
         if dtype not in _DT:
             raise TypeError(f"mx_dequantize: {dtype} is not float32, bfloat16 or float16")
-        out = torch.empty((rows.num_units, rows.batch), dtype=dtype, device=rows.device)
+        out = rows.codes.new_empty((rows.num_units, rows.batch), dtype=dtype)
     else:
         if out.dtype not in _DT:
             raise TypeError(f"mx_dequantize: out is {out.dtype}, expected float32, bfloat16 or float16")
@@ -252,7 +263,7 @@ def mx_edge_grad(bucket: K.Bucket, grad: torch.Tensor, act: MxRows, *, out: torc
     float32 [capacity], 0 for dead slots."""
     cap = _edge_args(bucket, grad, act, "mx_edge_grad")
     if out is None:
-        out = torch.empty(cap, dtype=torch.float32, device=act.device)
+        out = grad.new_empty(cap)
     else:
         _tensor(out, torch.float32, (cap,), "mx_edge_grad: out", act.device)
     _launch(act.device, "pxb_mx_edge_grad", cap, K.ptr(bucket["from_id"]), K.ptr(bucket["to_id"]), K.ptr(bucket["dead"]),
@@ -296,24 +307,28 @@ class MxConns:
     scales: torch.Tensor | None = None
 
     def __post_init__(self) -> None:
-        fmt = _format(self.weights, (*FORMATS, "f32"), "weight format")
-        dev = self.units.device
-        m, e = self.units.numel(), self.src.numel()
-        _tensor(self.units, torch.int32, (m,), "MxConns.units")
-        _tensor(self.offsets, torch.int64, (m + 1,), "MxConns.offsets", dev)
-        _tensor(self.src, torch.int32, (e,), "MxConns.src", dev)
-        blocks = 0
+        fmt = _format(self.weights, WEIGHT_FORMATS, "weight format")
+        units, offsets, src = self.units, self.offsets, self.src
+        dev, m, e = units.device, units.numel(), src.numel()
+        _tensor(units, torch.int32, (m,), "MxConns.units")
+        _tensor(offsets, torch.int64, (m + 1,), "MxConns.offsets", dev)
+        _tensor(src, torch.int32, (e,), "MxConns.src", dev)
         if self.weights == "f32":
             _tensor(self.weight, torch.float32, (e,), "MxConns.weight", dev)
+            c = _lib.MxConns(m, fmt, e, 0, units.data_ptr(), offsets.data_ptr(), src.data_ptr(), self.weight.data_ptr(),
+                             None, None, None)
         else:
             _tensor(self.block_offsets, torch.int64, (m + 1,), "MxConns.block_offsets", dev)
-            _tensor(self.scales, torch.uint8, None, "MxConns.scales", dev)
+            _tensor(self.scales, _U8, None, "MxConns.scales", dev)
             blocks = self.scales.numel()
-            _tensor(self.scales, torch.uint8, (blocks,), "MxConns.scales")
-            _tensor(self.codes, torch.uint8, (blocks, block_bytes(self.weights)), "MxConns.codes", dev)
-        object.__setattr__(self, "_c", _lib.MxConns(
-            m, fmt, e, blocks, *(None if t is None else t.data_ptr() for t in (
-                self.units, self.offsets, self.src, self.weight, self.block_offsets, self.codes, self.scales))))
+            if self.scales.dim() != 1:
+                raise ValueError(f"MxConns.scales: expected shape {(blocks,)}, got {tuple(self.scales.shape)}")
+            _tensor(self.codes, _U8, (blocks, block_bytes(self.weights)), "MxConns.codes", dev)
+            if self.codes.data_ptr() % 16:
+                raise ValueError("MxConns.codes: must start on a 16-byte boundary")
+            c = _lib.MxConns(m, fmt, e, blocks, units.data_ptr(), offsets.data_ptr(), src.data_ptr(), None,
+                             self.block_offsets.data_ptr(), self.codes.data_ptr(), self.scales.data_ptr())
+        object.__setattr__(self, "_c", c)
 
     @property
     def num_edges(self) -> int:
@@ -326,7 +341,7 @@ class MxConns:
         destination, in their order, and lay their weights out. Edges into
         other units are left out. Setup: sorts and sizes on the device, and
         reads counts on the host."""
-        _format(weights, (*FORMATS, "f32"), "weight format")
+        _format(weights, WEIGHT_FORMATS, "weight format")
         dev, m = units.device, units.numel()
         ids = units.long()
         at = torch.searchsorted(ids, dst.long())

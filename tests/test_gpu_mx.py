@@ -396,6 +396,87 @@ def test_product(cuda, rows, weights, degrees, batch):
         _same(q, *[np.where(left[:, None], v, r) for v, r in zip((1, 2), _mx.quantize(got, fmt))])
 
 
+@pytest.mark.parametrize("weights", [*FMTS, "f32"])
+@pytest.mark.parametrize("batch", [1, 2, 3, 4, 5])
+def test_product_of_many_short_destinations(cuda, weights, batch):
+    """Float32 rows of few samples and enough destinations that several share
+    a warp (five samples: the form beside it)."""
+    rng = np.random.default_rng(batch)
+    degrees = rng.integers(0, 75, 11003)
+    degrees[rng.random(degrees.size) < 0.2] = 0
+    num_src = 300
+    conns, off, src, w, units = _graph(rng, degrees, num_src, weights, cuda)
+    src[::97] = -5
+    src[50::101] = num_src
+    conns.src.copy_(torch.from_numpy(src))
+    x = _values(rng, num_src, batch).clip(-50, 50)
+    total = len(units) + 4
+    kind = ["identity", "tanh", "relu", "sigmoid"][batch % 4]
+    y, err = _mx.product(off, src, w, x.astype(np.float64), units, total, kind, num_src)
+    left = np.ones(total, bool)
+    left[units] = False
+    out = torch.full((total, batch), 7.0, device=cuda)
+    px.mx_product(conns, torch.from_numpy(x).to(cuda), activation=kind, out=out)
+    got = out.cpu().numpy()
+    assert (got[left] == 7).all()
+    _within(got[~left], y[~left], err[~left])
+    for fmt in FMTS:
+        q = px.MxRows.empty(total, batch, fmt, cuda)
+        q.codes.fill_(1), q.scales.fill_(2)
+        px.mx_product(conns, torch.from_numpy(x).to(cuda), activation=kind, out=q)
+        _same(q, *[np.where(left[:, None], v, r) for v, r in zip((1, 2), _mx.quantize(got, fmt))])
+
+
+def test_rows_past_four_gigabytes(cuda):
+    """Row offsets that do not fit 32 bits: the last rows of float32 rows and of
+    8-bit rows that end past 4 GiB, through every operator that indexes rows."""
+    rng = np.random.default_rng(2)
+    batch, n = 1024, (1 << 20) + 4096  # 4.3 GB of float32
+    pick = np.array([0, 5, n - 2, n - 1])
+    few = rng.standard_normal((4, batch)).astype(np.float32)
+    x = torch.zeros((n, batch), device=cuda)
+    ids = torch.from_numpy(pick).to(cuda)
+    x[ids] = torch.from_numpy(few).to(cuda)
+    conns = px.MxConns(torch.tensor([n - 3, 1], dtype=torch.int32, device=cuda), torch.tensor([0, 3, 4], device=cuda),
+                       torch.tensor([5, n - 1, n - 2, n - 1], dtype=torch.int32, device=cuda), "f32",
+                       weight=torch.tensor([1.0, 2.0, -0.5, 3.0], device=cuda))
+    px.mx_product(conns, x, out=x)  # no destination is a source
+    want = few[1].astype(np.float64) + 2.0 * few[3] - 0.5 * few[2]
+    got = x[torch.tensor([n - 3, 1], device=cuda)].cpu().numpy()
+    bound = 5 * _mx.U32 * (np.abs(few[1]) + 2 * np.abs(few[3]) + np.abs(few[2]))
+    assert (np.abs(got[0] - want) <= bound).all() and np.array_equal(got[1], np.float32(3.0) * few[3])
+    # quantised rows and their gradient
+    ck = px.mx_quantize(x, "e4m3", keep_nonzero=True)
+    codes, scales = _mx.quantize(few, "e4m3", True)
+    np.testing.assert_array_equal(ck.codes[ids].cpu().numpy(), codes)
+    np.testing.assert_array_equal(ck.scales[ids].cpu().numpy(), scales)
+    a = _mx.values(codes, scales, "e4m3", batch)
+    f, t = np.array([0, 3, 2, 1, 3]), np.array([3, 2, 3, 0, 0])
+    bucket = {"from_id": torch.from_numpy(pick[f].astype(np.int32)).to(cuda),
+              "to_id": torch.from_numpy(pick[t].astype(np.int32)).to(cuda),
+              "dead": torch.zeros(5, dtype=torch.uint8, device=cuda)}
+    out = px.mx_edge_grad(bucket, x, ck).cpu().numpy()
+    prod = few[t].astype(np.float64) * a[f]
+    assert (np.abs(out - prod.sum(1) / batch) <= (batch + 4) * _mx.U32 * np.abs(prod).sum(1) / batch).all()
+    g = px.mx_unit_grad(x, ck, "tanh", out=x)[ids].cpu().numpy()
+    up = few.astype(np.float64)
+    assert (np.abs(g - up * (1 - a * a)) <= 4 * _mx.U32 * np.abs(up) * (1 + a * a)).all()
+    back = px.mx_dequantize(ck)
+    np.testing.assert_array_equal(back[ids].cpu().numpy(), a.astype(np.float32))
+    del x, ck, back
+    # 8-bit rows past 4 GiB
+    n = (1 << 22) + 4096
+    rows = px.MxRows.empty(n, batch, "e4m3", cuda, zero=True)
+    ids = torch.tensor([n - 1, n - 2, 0, 7], device=cuda)
+    px.mx_quantize(torch.from_numpy(few).to(cuda), "e4m3", keep_nonzero=True, ids=ids, out=rows)
+    np.testing.assert_array_equal(rows.codes[ids].cpu().numpy(), codes)
+    conns = px.MxConns(torch.tensor([0], dtype=torch.int32, device=cuda), torch.tensor([0, 2], device=cuda),
+                       torch.tensor([n - 1, n - 2], dtype=torch.int32, device=cuda), "f32",
+                       weight=torch.tensor([1.5, -1.0], device=cuda))
+    out = px.mx_product(conns, rows, out=torch.zeros((1, batch), device=cuda)).cpu().numpy()[0]
+    assert (np.abs(out - (1.5 * a[0] - a[1])) <= 4 * _mx.U32 * (1.5 * np.abs(a[0]) + np.abs(a[1]))).all()
+
+
 def test_product_skips_what_is_out_of_range(cuda):
     rng = np.random.default_rng(1)
     conns, off, src, w, units = _graph(rng, [10, 40, 3], 20, "e2m1", cuda)

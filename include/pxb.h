@@ -309,8 +309,8 @@ PXB_API int pxb_batched_update(int64_t cap, const int32_t *from_id,
 /* ------------------------------------------------------------------ */
 
 /* A row of `batch` samples of one unit is ceil(batch / 32) blocks. A block is
- * one scale byte (2^(byte - 127); 255: the block is not a number) and 32
- * codes: 32 bytes of e4m3 or e5m2, or 16 bytes of e2m1 (the even sample in
+ * one scale byte (2^(byte - 127); 255: the block is not a number, and its
+ * codes are 0) and 32 codes: 32 bytes of e4m3 or e5m2, or 16 bytes of e2m1 (the even sample in
  * the low nibble). Rows of codes are [num_units, blocks * 32 or 16] bytes,
  * 16-byte aligned; rows of scales [num_units, blocks] bytes. The samples past
  * `batch` in the last block are code 0.

@@ -90,6 +90,28 @@ __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
   return same_bits<float2>(d);
 }
 
+// Sums over the lanes OFF, OFF / 2, ... LANES apart: half of the N values left go
+// to the other side each time, until one is left; a lane ends with the values
+// from `base` on.
+template <int OFF, int LANES, int N, int A>
+__device__ __forceinline__ void fold_lanes(float (&f)[A], int lane, int &base) {
+  if constexpr (OFF >= LANES && OFF > 0) {
+    if constexpr (N > 1) {
+      const bool upper = (lane & OFF) != 0;
+#pragma unroll
+      for (int q = 0; q < N / 2; ++q) {
+        const float send = upper ? f[q] : f[q + N / 2], keep = upper ? f[q + N / 2] : f[q];
+        f[q] = keep + __shfl_xor_sync(0xffffffffu, send, OFF);
+      }
+      base += upper ? N / 2 : 0;
+      fold_lanes<OFF / 2, LANES, N / 2>(f, lane, base);
+    } else {
+      f[0] += __shfl_xor_sync(0xffffffffu, f[0], OFF);
+      fold_lanes<OFF / 2, LANES, 1>(f, lane, base);
+    }
+  }
+}
+
 // One slice of slot_sums: the group's eight slots' products into p. UNIFORM:
 // their source is `f` for the whole group.
 template <int FMT, bool VEC, bool FULL, bool UNIFORM, int DEPTH, typename O>
@@ -153,15 +175,8 @@ __device__ __forceinline__ float slot_sums(const EdgeGrad &k, const Slot &slot, 
   float q[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) q[j] = p[j].x + p[j].y;
-#pragma unroll
-  for (int half = 4; half > 0; half >>= 1) {
-    const bool upper = (lane & half) != 0;
-#pragma unroll
-    for (int i = 0; i < half; ++i) {
-      const float send = upper ? q[i] : q[i + half], keep = upper ? q[i + half] : q[i];
-      q[i] = keep + __shfl_xor_sync(0xffffffffu, send, half);
-    }
-  }
+  int which = 0;
+  fold_lanes<4, 1, 8>(q, lane, which);
   return q[0];
 }
 
@@ -406,19 +421,17 @@ struct Piece {
   float w;
 };
 
-// Offsets of rows in bytes; one past every row where the edge has no source.
-template <typename O>
-constexpr O kNoRow = ~O(0);
-
+// A piece of the row at byte offset `row` for an edge of weight w. `valid`:
+// the edge has a source; where not, `row` is 0, whose values the factor 0 (for
+// e2m1, whose codes are all finite) or zeros in their place leave out.
 template <int XF, bool VEC, typename O>
-__device__ __forceinline__ Piece<XF> load_piece(const Rows &r, O row, float w, int32_t piece, bool on) {
+__device__ __forceinline__ Piece<XF> load_piece(const Rows &r, O row, float w, bool valid, int32_t piece) {
   Piece<XF> p;
-  p.v = make_uint4(0, 0, 0, 0);
-  p.w = 0.0f;
-  if (!on || row == kNoRow<O>) return p;
   if constexpr (XF == PXB_MX_F32) {
+    p.v = make_uint4(0, 0, 0, 0);
+    p.w = valid ? w : 0.0f;
+    if (!valid) return p;
     const float *x = reinterpret_cast<const float *>(reinterpret_cast<const char *>(r.x) + row) + piece * 4;
-    p.w = w;
     if (VEC) {
       p.v = __ldg(reinterpret_cast<const uint4 *>(x));
     } else {
@@ -432,7 +445,11 @@ __device__ __forceinline__ Piece<XF> load_piece(const Rows &r, O row, float w, i
   } else {
     constexpr int kShift = XF == PXB_MX_E2M1 ? 4 : 5;  // a block's bytes of codes
     p.v = __ldg(reinterpret_cast<const uint4 *>(r.codes + row) + piece);
-    p.w = __fmul_rn(w, mx_scale_value(__ldg(r.scales + (row >> kShift) + (piece >> (kShift - 4)))));
+    const uint32_t s = __ldg(r.scales + (row >> kShift) + (piece >> (kShift - 4)));
+    // as mx_scale_value, but for 255: infinite, which the block's codes, 0, make not a number
+    const float f = __fmul_rn(w, __uint_as_float(max(s << 23, 0x00400000u)));
+    p.w = valid ? f : 0.0f;
+    if (XF != PXB_MX_E2M1 && !valid) p.v = make_uint4(0, 0, 0, 0);
   }
   return p;
 }
@@ -484,8 +501,7 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
     for (int q = 0; q < A / 2; ++q) acc[q] = make_float2(0.0f, 0.0f);
     if (item < n.total) {
       const Item it = load_item(c, n, item);
-      const int32_t piece = it.chunk * LANES + sub;
-      const bool on = piece < pieces;
+      const int32_t piece = min(it.chunk * LANES + sub, pieces - 1);  // past the row: the last again, its sums unread
       int32_t k = member + rank * n.wpd;
       if constexpr (LANES == 1) {  // four blocks at once: a lane's edge has one piece
 #pragma unroll 1
@@ -497,7 +513,7 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
           for (int d = 0; d < 4; ++d) load_edge(c, it, k + d * step, lane, r.rows, s[d], w[d]);
 #pragma unroll
           for (int d = 0; d < 4; ++d)
-            p[d] = load_piece<XF, VEC, O>(r, s[d] < 0 ? kNoRow<O> : static_cast<O>(s[d]) * row_bytes, w[d], piece, on);
+            p[d] = load_piece<XF, VEC, O>(r, s[d] < 0 ? O(0) : static_cast<O>(s[d]) * row_bytes, w[d], s[d] >= 0, piece);
 #pragma unroll
           for (int d = 0; d < 4; ++d) add_piece<XF>(p[d], acc);
         }
@@ -507,7 +523,8 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
       load_edge(c, it, k, lane, r.rows, next, next_w);
 #pragma unroll 1
       for (; k < it.blocks; k += step) {
-        const O row = next < 0 ? kNoRow<O> : static_cast<O>(next) * row_bytes;
+        const O row = next < 0 ? O(0) : static_cast<O>(next) * row_bytes;
+        const unsigned valid = __ballot_sync(0xffffffffu, next >= 0);
         const float w = next_w;
         load_edge(c, it, k + step, lane, r.rows, next, next_w);
         const int cnt = k == it.blocks - 1 ? it.tail : 32;
@@ -517,34 +534,21 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
 #pragma unroll
           for (int d = 0; d < kDepth; ++d) {
             const int at = j + d * kGroups + grp;
-            p[d] = load_piece<XF, VEC, O>(r, __shfl_sync(0xffffffffu, row, at), __shfl_sync(0xffffffffu, w, at), piece, on);
+            p[d] = load_piece<XF, VEC, O>(r, __shfl_sync(0xffffffffu, row, at), __shfl_sync(0xffffffffu, w, at),
+                                          (valid >> at) & 1, piece);
           }
 #pragma unroll
           for (int d = 0; d < kDepth; ++d) add_piece<XF>(p[d], acc);
         }
       }
     }
-    // the edges read side by side join: halves of the samples go to the other side until one is left
+    // the edges read side by side join
     float f[A];
 #pragma unroll
     for (int q = 0; q < A / 2; ++q) f[2 * q] = acc[q].x, f[2 * q + 1] = acc[q].y;
     int base = sub * A;
+    fold_lanes<16, LANES, A>(f, lane, base);
     constexpr int kHeld = A > kGroups ? A / kGroups : 1;
-#pragma unroll
-    for (int off = 16, left = A; off >= LANES; off >>= 1) {
-      if (left > 1) {
-        left >>= 1;
-        const bool upper = (lane & off) != 0;
-#pragma unroll
-        for (int q = 0; q < left; ++q) {
-          const float send = upper ? f[q] : f[q + left], keep = upper ? f[q + left] : f[q];
-          f[q] = keep + __shfl_xor_sync(0xffffffffu, send, off);
-        }
-        base += upper ? left : 0;
-      } else {
-        f[0] += __shfl_xor_sync(0xffffffffu, f[0], off);
-      }
-    }
 #pragma unroll
     for (int q = 0; q < kHeld; ++q) part[warp][base + q] = f[q];
     finish_items<kChunk>(c, r, act_kind, out, n, tile, ranks, &part[0][0], kChunk);
@@ -784,7 +788,7 @@ extern "C" int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src, int32_
   PXB_REQUIRE(out_fmt == PXB_MX_F32 ? out != nullptr : out_codes && out_scales, "pxb_mx_product: out is NULL");
   PXB_REQUIRE(aligned16(x_codes) && aligned16(out_codes) && aligned16(conns->codes),
               "pxb_mx_product: codes must be 16-byte aligned");
-  const Conns c{conns->num_dst, conns->fmt, conns->num_edges, conns->num_blocks, conns->units, conns->offsets, conns->src,
+  const Conns c{conns->num_dst, conns->fmt, num_src > 0 ? conns->num_edges : 0, conns->num_blocks, conns->units, conns->offsets, conns->src,
                 conns->weight, conns->block_offsets, conns->codes, conns->scales};
   const int32_t nb = static_cast<int32_t>(mx_blocks(batch));
   cudaStream_t st = as_stream(stream);

@@ -266,7 +266,8 @@ def mx_edge_grad(bucket: K.Bucket, grad: torch.Tensor, act: MxRows, *, out: torc
         out = grad.new_empty(cap)
     else:
         _tensor(out, torch.float32, (cap,), "mx_edge_grad: out", act.device)
-    _launch(act.device, "pxb_mx_edge_grad", cap, K.ptr(bucket["from_id"]), K.ptr(bucket["to_id"]), K.ptr(bucket["dead"]),
+    _launch(act.device, "pxb_mx_edge_grad", cap, bucket["from_id"].data_ptr(),
+            bucket["to_id"].data_ptr(), bucket["dead"].data_ptr(),
             grad.data_ptr(), act.codes.data_ptr(), act.scales.data_ptr(), _lib.MX[act.fmt], act.batch,
             act.num_units, out.data_ptr(), None, None, None, None, None)
     return out
@@ -280,9 +281,10 @@ def mx_update(bucket: K.Bucket, grad: torch.Tensor, act: MxRows, opt: _lib.Optim
     for name in ("weight", "opt/m", "opt/v", "opt/t"):
         if name == "weight" or name in bucket:
             _tensor(bucket[name], torch.float32, (cap,), f"mx_update: bucket column {name!r}", act.device)
-    _launch(act.device, "pxb_mx_edge_grad", cap, K.ptr(bucket["from_id"]), K.ptr(bucket["to_id"]), K.ptr(bucket["dead"]),
+    _launch(act.device, "pxb_mx_edge_grad", cap, bucket["from_id"].data_ptr(),
+            bucket["to_id"].data_ptr(), bucket["dead"].data_ptr(),
             grad.data_ptr(), act.codes.data_ptr(), act.scales.data_ptr(), _lib.MX[act.fmt], act.batch,
-            act.num_units, None, K.ptr(bucket["weight"]), ctypes.byref(opt), K.ptr(bucket.get("opt/m")),
+            act.num_units, None, bucket["weight"].data_ptr(), ctypes.byref(opt), K.ptr(bucket.get("opt/m")),
             K.ptr(bucket.get("opt/v")), K.ptr(bucket.get("opt/t")))
 
 

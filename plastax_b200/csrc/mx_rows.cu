@@ -173,19 +173,20 @@ __device__ __forceinline__ void settle(const Grid &g, const Octet &o, const Raw<
     }
   } else {
     const int lane = threadIdx.x & 31;
+    T *b = reinterpret_cast<T *>(buf);
     __syncwarp();
 #pragma unroll
     for (int q = 0; q < Moves<LAYOUT>::kMoves; ++q) {
-      if constexpr (LAYOUT == RUN2) {
-        const auto h = same_bits<Pack<T, 2>>(r.v[q]);
-        reinterpret_cast<float2 *>(buf)[q * 32 + lane] = make_float2(to_f32(h.v[0]), to_f32(h.v[1]));
-      } else {
-        buf[q * 32 + lane] = to_f32(r.v[q]);
-      }
+      if constexpr (LAYOUT == RUN2) reinterpret_cast<uint32_t *>(b)[q * 32 + lane] = r.v[q];
+      else b[q * 32 + lane] = r.v[q];
     }
     __syncwarp();
-    const float4 a = reinterpret_cast<const float4 *>(buf)[lane * 2], b = reinterpret_cast<const float4 *>(buf)[lane * 2 + 1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q) {
+      const auto h = same_bits<Pack<T, 16 / sizeof(T)>>(reinterpret_cast<const uint4 *>(b)[lane * (sizeof(T) / 2) + q]);
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) v[q * (16 / sizeof(T)) + i] = to_f32(h.v[i]);
+    }
   }
 }
 
@@ -196,16 +197,22 @@ __device__ __forceinline__ void put(const Grid &g, uint32_t tile, const Octet &o
                                     float *buf, const float (&v)[8]) {
   if constexpr (LAYOUT != ALIGNED) {
     const int lane = threadIdx.x & 31;
+    T *b = reinterpret_cast<T *>(buf);
     __syncwarp();
-    reinterpret_cast<float4 *>(buf)[lane * 2] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(buf)[lane * 2 + 1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(sizeof(T) / 2); ++q) {
+      Pack<T, 16 / sizeof(T)> h;
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) h.v[i] = from_f32<T>(v[q * (16 / sizeof(T)) + i]);
+      reinterpret_cast<uint4 *>(b)[lane * (sizeof(T) / 2) + q] = same_bits<uint4>(h);
+    }
     __syncwarp();
     const Moves<LAYOUT> m(g, tile, lane);
     if constexpr (LAYOUT == TILE) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const uint32_t u = m.u(q);
-        if (u < static_cast<uint32_t>(g.rows) && m.b(q) < g.batch && keep(u)) out[u * ld + m.b(q)] = from_f32<T>(buf[q * 32 + lane]);
+        if (u < static_cast<uint32_t>(g.rows) && m.b(q) < g.batch && keep(u)) out[u * ld + m.b(q)] = b[q * 32 + lane];
       }
     } else {
       const int32_t end = m.u0 < static_cast<uint32_t>(g.rows) && keep(m.u0) ? g.batch : 0;
@@ -213,12 +220,11 @@ __device__ __forceinline__ void put(const Grid &g, uint32_t tile, const Octet &o
 #pragma unroll
       for (int q = 0; q < Moves<LAYOUT>::kMoves; ++q) {
         if constexpr (LAYOUT == RUN) {
-          if (m.b(q) < end) p[q * 32] = from_f32<T>(buf[q * 32 + lane]);
+          if (m.b(q) < end) p[q * 32] = b[q * 32 + lane];
         } else {
-          const float2 two = reinterpret_cast<const float2 *>(buf)[q * 32 + lane];
-          const Pack<T, 2> h{from_f32<T>(two.x), from_f32<T>(two.y)};
-          if (m.b(q) < (end & ~1)) *reinterpret_cast<uint32_t *>(p + q * 64) = same_bits<uint32_t>(h);
-          if ((end & 1) && m.b(q) == end - 1) p[q * 64] = h.v[0];
+          const uint32_t two = reinterpret_cast<const uint32_t *>(b)[q * 32 + lane];
+          if (m.b(q) < (end & ~1)) *reinterpret_cast<uint32_t *>(p + q * 64) = two;
+          if ((end & 1) && m.b(q) == end - 1) p[q * 64] = same_bits<Pack<T, 2>>(two).v[0];
         }
       }
     }

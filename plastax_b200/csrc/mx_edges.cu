@@ -555,18 +555,24 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
   }
 }
 
-// Up to four samples of float32 rows and many short destinations: eight lanes a
-// destination, four consecutive edges of a weight block each (their codes are
-// one load, their scale one), so a warp works on four destinations and the
-// set-up and the ending of each cost a quarter of a warp's. One sample of 32,768
-// destinations of 64 in-edges: 27 us with a warp each, 10 with eight lanes.
+// Up to 16 samples (4 * Q) of float32 rows and many short destinations: eight
+// lanes a destination, four consecutive edges of a weight block each (their
+// codes are one load, their scale one), so a warp works on four destinations
+// and the set-up and the ending of each cost a quarter of a warp's. 32,768
+// destinations of 64 in-edges: one sample 10 us against 27 with a warp each,
+// eight samples 18 against 38, 16 samples 34 against 42 (rows that need single
+// loads: 13 samples 52 against 44, so past eight samples only whole vectors).
+template <int Q, bool VEC>
 __global__ void __launch_bounds__(256) mx_product_short_kernel(Conns c, Rows r, int act_kind, Out out) {
-  const int sub = threadIdx.x & 7;
+  constexpr int N = 4 * Q;
+  const int lane = threadIdx.x & 31, sub = lane & 7;
   const int64_t teams = static_cast<int64_t>(gridDim.x) * 32;
   // whole warps step together (the shuffles below take every lane)
   for (int64_t i0 = (blockIdx.x * int64_t(256) + threadIdx.x) / 32 * 4; i0 < c.num_dst; i0 += teams) {
-    const int64_t i = i0 + ((threadIdx.x & 31) >> 3);
-    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    const int64_t i = i0 + (lane >> 3);
+    float f[N];
+#pragma unroll
+    for (int b = 0; b < N; ++b) f[b] = 0.0f;
     if (i < c.num_dst) {
       const int64_t e0 = max(int64_t(0), __ldg(c.offsets + i)), e1 = min(c.num_edges, __ldg(c.offsets + i + 1));
       int64_t blk = c.fmt == PXB_MX_F32 ? 0 : max(int64_t(0), __ldg(c.block_offsets + i));
@@ -594,50 +600,70 @@ __global__ void __launch_bounds__(256) mx_product_short_kernel(Conns c, Rows r, 
           w[0] = __fmul_rn(lo.x, scale), w[1] = __fmul_rn(lo.y, scale);
           w[2] = __fmul_rn(hi.x, scale), w[3] = __fmul_rn(hi.y, scale);
         }
-        float x[4][4];
+        constexpr int kAtOnce = Q == 4 ? 2 : 4;  // edges whose rows are in flight together
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const bool on = static_cast<uint32_t>(s[q]) < r.rows;
-          const float *p = r.x + static_cast<int64_t>(s[q]) * r.batch;
-          if (!on) w[q] = 0.0f;
+        for (int q0 = 0; q0 < 4; q0 += kAtOnce) {
+          float x[kAtOnce][N];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) x[q][b] = on && b < r.batch ? __ldg(p + b) : 0.0f;
+          for (int q = 0; q < kAtOnce; ++q) {
+            const bool on = static_cast<uint32_t>(s[q0 + q]) < r.rows;
+            const float *p = r.x + static_cast<int64_t>(on ? s[q0 + q] : 0) * r.batch;
+            if (!on) w[q0 + q] = 0.0f;
+            if constexpr (VEC) {
+#pragma unroll
+              for (int z = 0; z < Q; ++z) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (on && z * 4 < r.batch) v = __ldg(reinterpret_cast<const float4 *>(p) + z);
+                x[q][4 * z] = v.x, x[q][4 * z + 1] = v.y, x[q][4 * z + 2] = v.z, x[q][4 * z + 3] = v.w;
+              }
+            } else {
+#pragma unroll
+              for (int b = 0; b < N; ++b) x[q][b] = on && b < r.batch ? __ldg(p + b) : 0.0f;
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+            for (int b = 0; b < N; ++b) f[b] = fmaf(w[q0 + q], x[q][b], f[b]);
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int b = 0; b < 4; ++b) f[b] = fmaf(w[q], x[q][b], f[b]);
       }
     }
-#pragma unroll
-    for (int off = 1; off < 8; off <<= 1)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) f[b] += __shfl_xor_sync(0xffffffffu, f[b], off);
     const int32_t u = i < c.num_dst ? __ldg(c.units + i) : -1;
-    if (static_cast<uint32_t>(u) >= out.rows) continue;
+    const bool on = static_cast<uint32_t>(u) < out.rows;
     if (out.fmt == PXB_MX_F32) {
-      const float v = sub == 0 ? f[0] : sub == 1 ? f[1] : sub == 2 ? f[2] : f[3];
-      if (sub < r.batch) out.x[static_cast<int64_t>(u) * r.batch + sub] = act_fn(act_kind, v);
-    } else if (sub < 4) {  // the block's octets, all but the first without samples
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      int base = 0;
+      fold_lanes<4, 1, N>(f, lane, base);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) v[b] = b < r.batch ? act_fn(act_kind, f[b]) : 0.0f;
-      const uint32_t m = mx_amax8(v);
-      if (sub > 0) v[0] = v[1] = v[2] = v[3] = 0.0f;
-      const int64_t at = static_cast<int64_t>(u) * 4 + sub;
-      uint32_t sb;
-      if (out.fmt == PXB_MX_E2M1) {
-        sb = mx_scale_byte<PXB_MX_E2M1>(m);
-        mx_store8<PXB_MX_E2M1>(out.codes, at, mx_encode8<PXB_MX_E2M1>(v, sb, false));
-      } else if (out.fmt == PXB_MX_E4M3) {
-        sb = mx_scale_byte<PXB_MX_E4M3>(m);
-        mx_store8<PXB_MX_E4M3>(out.codes, at, mx_encode8<PXB_MX_E4M3>(v, sb, false));
-      } else {
-        sb = mx_scale_byte<PXB_MX_E5M2>(m);
-        mx_store8<PXB_MX_E5M2>(out.codes, at, mx_encode8<PXB_MX_E5M2>(v, sb, false));
-      }
-      if (sub == 0) out.scales[u] = static_cast<uint8_t>(sb);
+      for (int z = 0; z < (N > 8 ? N / 8 : 1); ++z)
+        if (on && base + z < r.batch) out.x[static_cast<int64_t>(u) * r.batch + base + z] = act_fn(act_kind, f[z]);
+      continue;
     }
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1)  // in fold_lanes' order: the same sums
+#pragma unroll
+      for (int b = 0; b < N; ++b) f[b] += __shfl_xor_sync(0xffffffffu, f[b], off);
+    if (!on || sub >= 4) continue;  // a lane an octet of the block
+    uint32_t m = 0;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < N; ++b) {
+      const float y = b < r.batch ? act_fn(act_kind, f[b]) : 0.0f;
+      m = max(m, __float_as_uint(y) & 0x7fffffffu);
+      if (sub == b / 8) v[b % 8] = y;
+    }
+    const int64_t at = static_cast<int64_t>(u) * 4 + sub;
+    uint32_t sb;
+    if (out.fmt == PXB_MX_E2M1) {
+      sb = mx_scale_byte<PXB_MX_E2M1>(m);
+      mx_store8<PXB_MX_E2M1>(out.codes, at, mx_encode8<PXB_MX_E2M1>(v, sb, false));
+    } else if (out.fmt == PXB_MX_E4M3) {
+      sb = mx_scale_byte<PXB_MX_E4M3>(m);
+      mx_store8<PXB_MX_E4M3>(out.codes, at, mx_encode8<PXB_MX_E4M3>(v, sb, false));
+    } else {
+      sb = mx_scale_byte<PXB_MX_E5M2>(m);
+      mx_store8<PXB_MX_E5M2>(out.codes, at, mx_encode8<PXB_MX_E5M2>(v, sb, false));
+    }
+    if (sub == 0) out.scales[u] = static_cast<uint8_t>(sb);
   }
 }
 
@@ -677,10 +703,15 @@ static int launch_items(const Conns &c, const Rows &r, int act, const Out &out, 
 
 template <int XF, int LANES>
 static int launch_product(const Conns &c, const Rows &r, int act, const Out &out, bool vec, cudaStream_t st) {
-  if constexpr (XF == PXB_MX_F32 && LANES == 1) {
+  if constexpr (XF == PXB_MX_F32 && (LANES == 1 || LANES == 2 || LANES == 4)) {
     // four short destinations a warp, as soon as that fills the SMs half
-    if (r.batch <= 4 && c.num_dst >= sm_count() * 64 && c.num_edges / c.num_dst <= 512) {
-      mx_product_short_kernel<<<mx_grid<mx_product_short_kernel>(c.num_dst, 32, 256), 256, 0, st>>>(c, r, act, out);
+    if ((LANES < 4 || vec) && r.batch <= 4 * LANES && c.num_dst >= sm_count() * 64 && c.num_edges / c.num_dst <= 512) {
+#define PXB_SHORT(V)                                                                                               \
+  mx_product_short_kernel<LANES, V>                                                                                \
+      <<<mx_grid<mx_product_short_kernel<LANES, V>>(c.num_dst, 32, 256), 256, 0, st>>>(c, r, act, out)
+      if (vec) PXB_SHORT(true);
+      else if constexpr (LANES < 4) PXB_SHORT(false);
+#undef PXB_SHORT
       PXB_LAUNCHED("mx_product_short_kernel");
       return PXB_OK;
     }

@@ -397,10 +397,10 @@ def test_product(cuda, rows, weights, degrees, batch):
 
 
 @pytest.mark.parametrize("weights", [*FMTS, "f32"])
-@pytest.mark.parametrize("batch", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("batch", [1, 2, 3, 4, 5, 8, 13, 16, 17])
 def test_product_of_many_short_destinations(cuda, weights, batch):
     """Float32 rows of few samples and enough destinations that several share
-    a warp (five samples: the form beside it)."""
+    a warp (17 samples: the form beside it)."""
     rng = np.random.default_rng(batch)
     degrees = rng.integers(0, 75, 11003)
     degrees[rng.random(degrees.size) < 0.2] = 0

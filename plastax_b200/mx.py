@@ -26,6 +26,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import dataclasses
+import functools
 
 import torch
 
@@ -65,10 +66,16 @@ def _on(dev: torch.device):
     return torch.cuda.device(dev)
 
 
+_entry = functools.cache(lambda name: getattr(_lib.lib(), name))
+
+
 def _launch(dev: torch.device, name: str, *args) -> None:
     """Call an entry point on `dev` and its current stream."""
-    if dev.type == "cuda" and dev.index == torch.cuda.current_device():
-        call(name, *args, K._stream())
+    i = dev.index
+    if dev.type == "cuda" and i == torch.cuda.current_device() and i == getattr(K._bound, "device", -1):
+        rc = _entry(name)(*args, K._raw_stream(i))  # the usual case, without a look-up twice
+        if rc != 0:
+            raise _lib.PxbError(f"{name} failed (status {rc}): {_lib.last_error()}")
         return
     with _on(dev):
         call(name, *args, K._stream())
@@ -92,9 +99,10 @@ def _tensor(t, dtype, shape, what: str, dev: torch.device | None = None) -> torc
 
 
 def _rows_shape(x: torch.Tensor, what: str) -> tuple[int, int]:
-    if x.dim() != 2:
-        raise ValueError(f"{what}: expected unit rows [num_units, batch], got shape {tuple(x.shape)}")
-    n, b = x.shape
+    shape = x.shape
+    if len(shape) != 2:
+        raise ValueError(f"{what}: expected unit rows [num_units, batch], got shape {tuple(shape)}")
+    n, b = shape
     if n >= 1 << 31 or b > _MAX_BATCH:
         raise ValueError(f"{what}: [{n}, {b}] is past 2^31 - 1 units or {_MAX_BATCH} samples")
     return n, b

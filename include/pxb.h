@@ -366,14 +366,19 @@ PXB_API int pxb_mx_unit_grad(int32_t num_units, int32_t batch,
  *   stat[s] = (sum_b g[to[s], b] * a[from[s], b]) / B   for live s,
  * summed in float32. With opt NULL, dw[s] = stat (0 for a dead slot, or one
  * whose ids are out of range); otherwise one optimizer step as
- * pxb_batched_update (dw must be NULL). Any batch >= 1. */
+ * pxb_batched_update (dw must be NULL). Any batch >= 1. `scratch` of
+ * pxb_mx_edge_grad_scratch_bytes (0 for most sizes) lets a small net's many
+ * slots share one matrix product; NULL: slot by slot. */
+PXB_API int pxb_mx_edge_grad_scratch_bytes(int64_t cap, int32_t batch,
+                                           int32_t num_units, size_t *bytes);
 PXB_API int pxb_mx_edge_grad(int64_t cap, const int32_t *from_id,
                              const int32_t *to_id, const uint8_t *dead,
                              const float *g, const uint8_t *codes,
                              const uint8_t *scales, int32_t fmt, int32_t batch,
                              int32_t num_units, float *dw, float *weight,
                              const pxb_optimizer *opt, float *opt_m,
-                             float *opt_v, float *opt_t, void *stream);
+                             float *opt_v, float *opt_t, void *scratch,
+                             size_t scratch_bytes, void *stream);
 
 /* In-edges grouped by destination: edges [offsets[i], offsets[i + 1]) of
  * `src` end in unit units[i]. Weights are float32 (fmt PXB_MX_F32: `weight`,

@@ -348,7 +348,8 @@ _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "pxb_mx_unit_grad": (c_i32, [c_i32, c_i32, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_ptr, c_i32, c_ptr, c_ptr,
                                  c_ptr]),
     "pxb_mx_edge_grad": (c_i32, [c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_i32, c_i32, c_ptr, c_ptr,
-                                 c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
+                                 c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr]),
+    "pxb_mx_edge_grad_scratch_bytes": (c_i32, [c_i64, c_i32, c_i32, ctypes.POINTER(c_size)]),
     "pxb_mx_product": (c_i32, [c_ptr, c_i32, c_i32, c_ptr, c_ptr, c_ptr, c_i32, c_i32, c_i32, c_ptr, c_ptr, c_ptr,
                                c_i32, c_ptr]),
     "pxb_propose_grid": (c_i32, [c_i32, c_i32, c_i32, c_i32, c_ptr, c_ptr, c_i32, c_ptr, c_ptr, c_ptr, c_i32, c_i32,

@@ -228,6 +228,187 @@ __global__ void __launch_bounds__(256) mx_edge_grad_split_kernel(EdgeGrad k) {
   cluster.sync();  // the peers have read this CTA's sums
 }
 
+// --- small nets, many edges ---------------------------------------------------
+// Where the slots are a good part of all pairs of units, every pair's sum is a
+// matrix product, D[t, f] = sum_b g[t, b] * a[f, b], and the slots pick theirs
+// from it. With 256 samples, us so and slot by slot: 400 x 300 units and 2^20
+// slots 15 and 74, 1000 x 1000 and 2^19 30 and 37 (43 partly regrown), 1000 x
+// 1000 and 300,000 28 and 25. An 8-bit activation is a bfloat16 exactly (four
+// significant bits, a power of two), and a float32 gradient is the sum of three
+// bfloat16 (8 + 8 + 8 bits), so three tensor-core products, added in float32,
+// hold what the float32 products do. Only the 64 x 64 tiles that some slot
+// touches are computed; the product lies in the caller's scratch, n^2 floats,
+// in L2. mma.sync is the bound of the middle kernel (tensor pipes 30 % busy over
+// its two rounds of tiles); the launches around it cost as much again.
+constexpr int kPairTile = 64, kPairUnits = 4096;
+
+__host__ __device__ inline int pair_tiles(uint32_t n) { return static_cast<int>((n + kPairTile - 1) / kPairTile); }
+
+// One bit a tile that some slot touches, by source tile, then target tile. A CTA
+// takes slots in a row (they share few sources) and gathers its bits in shared
+// memory, so few words reach L2 from it.
+__global__ void __launch_bounds__(512) mx_pair_mark_kernel(EdgeGrad k, uint32_t *__restrict__ marks) {
+  __shared__ uint32_t bits[kPairUnits / kPairTile * (kPairUnits / kPairTile) / 32];
+  const int tiles = pair_tiles(k.n), words = (tiles * tiles + 31) / 32;
+  for (int i = threadIdx.x; i < words; i += 512) bits[i] = 0;
+  __syncthreads();
+  const int64_t each = ((k.cap + gridDim.x - 1) / gridDim.x + 31) & ~int64_t(31);
+  const int64_t first = blockIdx.x * each, last = min(k.cap, first + each);
+  for (int64_t s = first + threadIdx.x; s < last; s += 512) {
+    const Slot slot = load_slot(k, s);
+    if (!slot.live(k.n)) continue;
+    const int at = slot.f / kPairTile * tiles + slot.t / kPairTile;
+    if ((bits[at >> 5] >> (at & 31) & 1) == 0) atomicOr(&bits[at >> 5], 1u << (at & 31));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < words; i += 512)
+    if (bits[i] != 0) atomicOr(marks + i, bits[i]);
+}
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const void *row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(row))) : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  return same_bits<uint32_t>(__floats2bfloat162_rn(lo, hi));
+}
+
+// Two gradients as their three bfloat16 parts (one that is not finite stands in
+// the first part alone).
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&p)[3]) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const float2 hf = __bfloat1622float2(h);
+  float rx = __fsub_rn(x, hf.x), ry = __fsub_rn(y, hf.y);
+  if (!isfinite(hf.x)) rx = 0.0f;
+  if (!isfinite(hf.y)) ry = 0.0f;
+  const __nv_bfloat162 m = __floats2bfloat162_rn(rx, ry);
+  const float2 mf = __bfloat1622float2(m);
+  p[0] = same_bits<uint32_t>(h);
+  p[1] = same_bits<uint32_t>(m);
+  p[2] = pack_bf16(__fsub_rn(rx, mf.x), __fsub_rn(ry, mf.y));
+}
+
+// A CTA of eight warps a tile; a warp 16 x 32 of it. 32 samples (a block) at a
+// time: the gradients' parts and the activations go to shared memory in
+// bfloat16 while the next block's words are on their way to registers. Rows of
+// 40 elements keep ldmatrix's eight rows on banks of their own.
+template <int FMT, bool VEC>
+__global__ void __launch_bounds__(256) mx_pair_product_kernel(EdgeGrad k, const uint32_t *__restrict__ marks,
+                                                              float *__restrict__ pairs) {
+  constexpr int kPitch = 40;
+  __shared__ __align__(16) uint16_t gs[3][kPairTile][kPitch], as[kPairTile][kPitch];
+  const int tiles = pair_tiles(k.n);
+  const int mark = blockIdx.x * tiles + blockIdx.y;
+  if (marks != nullptr && (marks[mark >> 5] >> (mark & 31) & 1) == 0) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t t0 = blockIdx.y * kPairTile, f0 = blockIdx.x * kPairTile;
+  const int wm = (warp >> 1) * 16, wn = (warp & 1) * 32;
+  // this thread's words of a block: two quads of gradients, rows tid / 8 + 32 i; eight codes, a quarter of a row
+  const int gq = tid & 7, gr = tid >> 3, ar = tid >> 2, aq = tid & 3;
+  const bool a_in = f0 + ar < k.n;
+  float4 g[2];
+  uint2 c;
+  uint32_t sc;
+  const auto fetch = [&](int32_t slice) {
+    const int32_t b = slice * kMxBlock + gq * 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t row = t0 + gr + 32 * i;
+      g[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < k.n) g[i] = load_grad<VEC, false, uint64_t>(k.g, (static_cast<uint64_t>(row) * k.batch + b) * 4, k.batch, b);
+    }
+    c = make_uint2(0, 0);
+    sc = 0;
+    if (a_in) {
+      const int64_t blk = static_cast<int64_t>(f0 + ar) * k.nb + slice;
+      c = __ldg(reinterpret_cast<const uint2 *>(k.codes) + blk * 4 + aq);
+      sc = __ldg(k.scales + blk);
+    }
+  };
+  float d[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.0f;
+  fetch(0);
+  for (int32_t slice = 0; slice < k.nb; ++slice) {
+    __syncthreads();  // the last block has been read
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t lo[3], hi[3];
+      split_bf16(g[i].x, g[i].y, lo);
+      split_bf16(g[i].z, g[i].w, hi);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<uint2 *>(&gs[p][gr + 32 * i][gq * 4]) = make_uint2(lo[p], hi[p]);
+    }
+    {
+      const float s = mx_scale_value(sc);
+      const uint32_t w[2] = {c.x, c.y};
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        __half2 h[2];
+        mx_decode_word<FMT>(w[i], h);
+        const float2 x = __half22float2(h[0]), y = __half22float2(h[1]);
+        o[2 * i] = pack_bf16(__fmul_rn(x.x, s), __fmul_rn(x.y, s));
+        o[2 * i + 1] = pack_bf16(__fmul_rn(y.x, s), __fmul_rn(y.y, s));
+      }
+      *reinterpret_cast<uint4 *>(&as[ar][aq * 8]) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    if (slice + 1 < k.nb) fetch(slice + 1);
+    __syncthreads();
+    // a block's sum by itself, then added with rounding: the tensor cores cut what lies below their largest addend's
+    // last bit, and over a whole batch in one accumulator that was 9 times a float32 sum's error (256 samples)
+    float e[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j][0] = e[j][1] = e[j][2] = e[j][3] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < kMxBlock; kk += 16) {
+      // B fragments of the warp's 32 columns: two loads of 16 columns x 16 samples
+      uint32_t b[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        ldmatrix_x4(b[j], &as[wn + j * 16 + (lane & 7) + ((lane >> 4) << 3)][kk + ((lane >> 3) & 1) * 8]);
+#pragma unroll
+      for (int p = 2; p >= 0; --p) {  // the smallest parts first
+        uint32_t a[4];
+        ldmatrix_x4(a, &gs[p][wm + (lane & 15)][kk + (lane >> 4) * 8]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma_bf16(e[j], a, b[j >> 1][(j & 1) * 2], b[j >> 1][(j & 1) * 2 + 1]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int z = 0; z < 4; ++z) d[j][z] += e[j][z];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t t = t0 + wm + (lane >> 2) + 8 * h, f = f0 + wn + j * 8 + (lane & 3) * 2;
+      if (t >= k.n) continue;
+      float *o = pairs + static_cast<int64_t>(t) * k.n + f;
+      if (f < k.n) o[0] = d[j][2 * h];
+      if (f + 1 < k.n) o[1] = d[j][2 * h + 1];
+    }
+}
+
+__global__ void __launch_bounds__(256) mx_pair_pick_kernel(EdgeGrad k, const float *__restrict__ pairs) {
+  for (int64_t s = blockIdx.x * int64_t(256) + threadIdx.x; s < k.cap; s += static_cast<int64_t>(gridDim.x) * 256) {
+    const Slot slot = load_slot(k, s);
+    const bool live = slot.live(k.n);
+    finish_slot(k, s, live, live ? __ldg(pairs + static_cast<int64_t>(slot.t) * k.n + slot.f) : 0.0f);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // out[units[i], :] = act(sum_e w[e] * x[src[e], :])
 // ---------------------------------------------------------------------------
@@ -732,6 +913,35 @@ static int launch_product(const Conns &c, const Rows &r, int act, const Out &out
               : launch_items<mx_product_kernel<XF, LANES, true, false>>(c, r, act, out, chunks, st);
 }
 
+// Scratch of the pair product (0 where slot by slot is as good): the pairs'
+// sums, then a bit a tile. At a twelfth of all pairs of units (between two
+// levels of a layered net a third or more of theirs) the two are alike; and
+// enough work to pay for four launches.
+static size_t pair_scratch(int64_t cap, int32_t batch, int64_t n) {
+  if (n > kPairUnits || cap * 12 < n * n || cap * batch < (int64_t(1) << 26)) return 0;
+  const int64_t tiles = pair_tiles(static_cast<uint32_t>(n));
+  return static_cast<size_t>(n * n * 4 + (tiles * tiles + 31) / 32 * 4);
+}
+
+template <int FMT, bool VEC>
+static int launch_pairs(const EdgeGrad &k, void *scratch, cudaStream_t st) {
+  float *pairs = static_cast<float *>(scratch);
+  uint32_t *marks = reinterpret_cast<uint32_t *>(pairs + static_cast<int64_t>(k.n) * k.n);
+  const int tiles = pair_tiles(k.n);
+  if (tiles * tiles <= sm_count()) {
+    marks = nullptr;  // a tile an SM at most: all of them
+  } else {
+    PXB_CUDA(cudaMemsetAsync(marks, 0, (static_cast<size_t>(tiles) * tiles + 31) / 32 * 4, st));
+    mx_pair_mark_kernel<<<grid_for(k.cap, 512, 2), 512, 0, st>>>(k, marks);
+    PXB_LAUNCHED("mx_pair_mark_kernel");
+  }
+  mx_pair_product_kernel<FMT, VEC><<<dim3(tiles, tiles), 256, 0, st>>>(k, marks, pairs);
+  PXB_LAUNCHED("mx_pair_product_kernel");
+  mx_pair_pick_kernel<<<grid_for(k.cap, 256, 8), 256, 0, st>>>(k, pairs);
+  PXB_LAUNCHED("mx_pair_pick_kernel");
+  return PXB_OK;
+}
+
 template <int FMT, bool VEC, bool WIDE>
 static int launch_edge_grad(const EdgeGrad &k, cudaStream_t st) {
   const int64_t blocks = (k.cap + 255) / 256;
@@ -765,7 +975,8 @@ using namespace pxb;
 extern "C" int pxb_mx_edge_grad(int64_t cap, const int32_t *from_id, const int32_t *to_id, const uint8_t *dead,
                                 const float *g, const uint8_t *codes, const uint8_t *scales, int32_t fmt,
                                 int32_t batch, int32_t num_units, float *dw, float *weight, const pxb_optimizer *opt,
-                                float *opt_m, float *opt_v, float *opt_t, void *stream) {
+                                float *opt_m, float *opt_v, float *opt_t, void *scratch, size_t scratch_bytes,
+                                void *stream) {
   PXB_REQUIRE(cap >= 0 && batch >= 1 && num_units >= 0, "pxb_mx_edge_grad: bad sizes");
   PXB_REQUIRE(fmt == PXB_MX_E4M3 || fmt == PXB_MX_E5M2, "pxb_mx_edge_grad: a checkpoint has 8 bits (e4m3 or e5m2)");
   if (cap == 0) return PXB_OK;
@@ -787,12 +998,31 @@ extern "C" int pxb_mx_edge_grad(int64_t cap, const int32_t *from_id, const int32
                    opt_v, opt_t};
   cudaStream_t st = as_stream(stream);
   const bool wide = !vec || static_cast<int64_t>(num_units) * batch * 4 >= (int64_t(1) << 32);
+  if (scratch != nullptr) {
+    const size_t need = pair_scratch(cap, batch, num_units);
+    if (scratch_bytes < need) {
+      set_error("pxb_mx_edge_grad: scratch of %zu bytes, %zu needed", scratch_bytes, need);
+      return PXB_ESCRATCH;
+    }
+    PXB_REQUIRE(aligned16(scratch), "pxb_mx_edge_grad: scratch must be 16-byte aligned");
+    if (need > 0) {
+      if (fmt == PXB_MX_E4M3) return vec ? launch_pairs<PXB_MX_E4M3, true>(k, scratch, st) : launch_pairs<PXB_MX_E4M3, false>(k, scratch, st);
+      return vec ? launch_pairs<PXB_MX_E5M2, true>(k, scratch, st) : launch_pairs<PXB_MX_E5M2, false>(k, scratch, st);
+    }
+  }
 #define PXB_EG(F) \
   return !vec ? launch_edge_grad<F, false, true>(k, st) \
               : wide ? launch_edge_grad<F, true, true>(k, st) : launch_edge_grad<F, true, false>(k, st)
   if (fmt == PXB_MX_E4M3) PXB_EG(PXB_MX_E4M3);
   PXB_EG(PXB_MX_E5M2);
 #undef PXB_EG
+}
+
+extern "C" int pxb_mx_edge_grad_scratch_bytes(int64_t cap, int32_t batch, int32_t num_units, size_t *bytes) {
+  PXB_REQUIRE(bytes != nullptr, "pxb_mx_edge_grad_scratch_bytes: bytes is NULL");
+  PXB_REQUIRE(cap >= 0 && batch >= 1 && num_units >= 0, "pxb_mx_edge_grad_scratch_bytes: bad sizes");
+  *bytes = num_units == 0 ? 0 : pair_scratch(cap, batch, num_units);
+  return PXB_OK;
 }
 
 extern "C" int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src, int32_t batch, const float *x,

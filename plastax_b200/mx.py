@@ -265,6 +265,18 @@ def _edge_args(bucket, grad: torch.Tensor, act: MxRows, what: str) -> int:
     return cap
 
 
+@functools.lru_cache(maxsize=256)
+def edge_grad_scratch_bytes(capacity: int, batch: int, num_units: int) -> int:
+    """Scratch that lets the gradient of a small net's many slots run as one
+    matrix product (0 for most sizes)."""
+    return _lib.query_size("pxb_mx_edge_grad_scratch_bytes", capacity, batch, num_units)
+
+
+def _scratch(act: MxRows, cap: int) -> tuple[torch.Tensor | None, int]:
+    size = edge_grad_scratch_bytes(cap, act.batch, act.num_units)
+    return (act.codes.new_empty(size), size) if size else (None, 0)
+
+
 def mx_edge_grad(bucket: K.Bucket, grad: torch.Tensor, act: MxRows, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """The batch-mean gradient of every slot of a bucket,
     (sum_b grad[to, b] * act[from, b]) / B, from checkpointed activations:
@@ -274,10 +286,11 @@ def mx_edge_grad(bucket: K.Bucket, grad: torch.Tensor, act: MxRows, *, out: torc
         out = grad.new_empty(cap)
     else:
         _tensor(out, torch.float32, (cap,), "mx_edge_grad: out", act.device)
+    scratch, size = _scratch(act, cap)
     _launch(act.device, "pxb_mx_edge_grad", cap, bucket["from_id"].data_ptr(),
             bucket["to_id"].data_ptr(), bucket["dead"].data_ptr(),
             grad.data_ptr(), act.codes.data_ptr(), act.scales.data_ptr(), _lib.MX[act.fmt], act.batch,
-            act.num_units, out.data_ptr(), None, None, None, None, None)
+            act.num_units, out.data_ptr(), None, None, None, None, None, K.ptr(scratch), size)
     return out
 
 
@@ -289,11 +302,12 @@ def mx_update(bucket: K.Bucket, grad: torch.Tensor, act: MxRows, opt: _lib.Optim
     for name in ("weight", "opt/m", "opt/v", "opt/t"):
         if name == "weight" or name in bucket:
             _tensor(bucket[name], torch.float32, (cap,), f"mx_update: bucket column {name!r}", act.device)
+    scratch, size = _scratch(act, cap)
     _launch(act.device, "pxb_mx_edge_grad", cap, bucket["from_id"].data_ptr(),
             bucket["to_id"].data_ptr(), bucket["dead"].data_ptr(),
             grad.data_ptr(), act.codes.data_ptr(), act.scales.data_ptr(), _lib.MX[act.fmt], act.batch,
             act.num_units, None, bucket["weight"].data_ptr(), ctypes.byref(opt), K.ptr(bucket.get("opt/m")),
-            K.ptr(bucket.get("opt/v")), K.ptr(bucket.get("opt/t")))
+            K.ptr(bucket.get("opt/v")), K.ptr(bucket.get("opt/t")), K.ptr(scratch), size)
 
 
 @dataclasses.dataclass(frozen=True)

@@ -258,6 +258,53 @@ def test_edge_grad(cuda, fmt, n, cap, batch):
     assert torch.equal(out, again)  # no order of summation to chance
 
 
+@pytest.mark.parametrize("fmt", mx.CHECKPOINT_FORMATS)
+@pytest.mark.parametrize("n,cap,batch", [(1, 1 << 21, 32), (64, 70001, 1001), (130, 262200, 256), (1000, 300000, 260),
+                                         (200, 2040000, 33)])
+def test_edge_grad_of_a_small_net_with_many_slots(cuda, fmt, n, cap, batch):
+    """The sizes that take one matrix product of all touched pairs: every
+    pair's sum in 64 bits, gathered; odd batches, edge tiles, bad ids, a NaN and
+    an infinity that reach their own row's slots only."""
+    assert mx.edge_grad_scratch_bytes(cap, batch, n) > 0
+    rng = np.random.default_rng(cap)
+    b, dev = _bucket(rng, n, cap, cuda)
+    g = (rng.standard_normal((n, batch)) * np.exp(rng.standard_normal((n, 1)) * 4)).astype(np.float32)
+    x = _values(rng, n, batch).clip(-100, 100)
+    if n > 5:
+        x[3, batch // 2] = np.nan
+        g[5, 1] = np.inf
+    ck = px.mx_quantize(torch.from_numpy(x).to(cuda), fmt, keep_nonzero=True)
+    a = _mx.values(ck.codes.cpu().numpy(), ck.scales.cpu().numpy(), fmt, batch)
+    f, t = b["from_id"].astype(np.int64), b["to_id"].astype(np.int64)
+    live = (b["dead"] == 0) & (f >= 0) & (f < n) & (t >= 0) & (t < n)
+    f, t = np.where(live, f, 0), np.where(live, t, 0)
+    with np.errstate(invalid="ignore"):
+        pairs, size = g.astype(np.float64) @ a.T / batch, np.abs(g).astype(np.float64) @ np.abs(a).T / batch
+    want, err = np.where(live, pairs[t, f], 0.0), np.where(live, size[t, f] * (batch + 4) * _mx.U32 * 1.01, 0.0)
+    got = px.mx_edge_grad(dev, torch.from_numpy(g).to(cuda), ck).cpu().numpy()
+    odd = ~np.isfinite(want)
+    if n > 5:  # the row with the infinity: infinite, or not a number where it meets a 0
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+        np.testing.assert_array_equal(got[np.isinf(want)], want[np.isinf(want)].astype(np.float32))
+        assert odd.any()
+    _within(got[~odd], want[~odd], err[~odd])
+    again = px.mx_edge_grad(dev, torch.from_numpy(g).to(cuda), ck, out=torch.full((cap,), 3.0, device=cuda)).cpu().numpy()
+    np.testing.assert_array_equal(got, again)
+
+
+def test_update_of_a_small_net_with_many_slots(cuda):
+    rng = np.random.default_rng(10)
+    n, cap, batch = 150, 262144, 256
+    b, dev = _bucket(rng, n, cap, cuda)
+    g = torch.from_numpy(rng.standard_normal((n, batch)).astype(np.float32)).to(cuda)
+    ck = px.mx_quantize(torch.from_numpy(rng.standard_normal((n, batch)).astype(np.float32)).to(cuda), "e4m3")
+    dw = px.mx_edge_grad(dev, g, ck)
+    w = torch.from_numpy(rng.standard_normal(cap).astype(np.float32)).to(cuda)
+    col = {**dev, "weight": w.clone()}
+    px.mx_update(col, g, ck, px.optim.sgd(0.25).struct())
+    assert torch.equal(col["weight"], w - 0.25 * dw)  # 0.25 dw is exact: one rounding on both sides
+
+
 def test_edge_grad_all_dead_empty_and_poisoned(cuda):
     rng = np.random.default_rng(8)
     b, dev = _bucket(rng, 10, 300, cuda, dead=0.0, bad=False)

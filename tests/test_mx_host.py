@@ -149,9 +149,16 @@ def test_abi_refuses_before_a_launch():
     refuse("pxb_mx_dequantize", 1, 32, 64, 64, 0, 64, 0, 31, None, text="overlap")
     refuse("pxb_mx_unit_apply", 1, 32, 0, 64, None, 0, None, 2, 64, 64, None, text="8 bits")
     refuse("pxb_mx_unit_grad", 1, 32, 9, 64, None, 64, 64, 0, None, 0, None, 64, None, text="activation")
-    refuse("pxb_mx_edge_grad", 8, 64, 64, 64, 64, 64, 64, 0, 0, 4, 64, None, None, None, None, None, None, text="sizes")
-    refuse("pxb_mx_edge_grad", 8, 64, 64, 64, 64, 64, 64, 0, 4, 4, None, None, None, None, None, None, None,
-           text="not both or neither")
+    refuse("pxb_mx_edge_grad", 8, 64, 64, 64, 64, 64, 64, 0, 0, 4, 64, None, None, None, None, None, None, 0,
+           None, text="sizes")
+    refuse("pxb_mx_edge_grad", 8, 64, 64, 64, 64, 64, 64, 0, 4, 4, None, None, None, None, None, None, None, 0,
+           None, text="not both or neither")
+    many = 1 << 20
+    assert lib.pxb_mx_edge_grad(many, 64, 64, 64, 64, 64, 64, 0, 256, 1000, 64, None, None, None, None, None, 64, 16,
+                                None) == 3 and "scratch" in _lib.last_error()
+    assert mx.edge_grad_scratch_bytes(many, 256, 1000) == 1000 * 1000 * 4 + 16 * 16 // 8
+    for sizes in ((many, 32, 1000), (many // 64, 256, 1000), (many, 256, 4097), (0, 1, 0)):
+        assert mx.edge_grad_scratch_bytes(*sizes) == 0
     conns = _lib.MxConns(2, 3, 4, 0, 64, 64, 64, None, None, None, None)
     import ctypes
 

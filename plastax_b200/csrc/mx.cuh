@@ -21,6 +21,7 @@
 namespace pxb {
 
 constexpr int kMxBlock = 32;
+constexpr int32_t kMxMaxBatch = 1 << 30;  // a row's padded samples stay within 32 bits
 
 // A value's bits as another type of its size.
 template <typename To, typename From>

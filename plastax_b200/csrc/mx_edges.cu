@@ -977,7 +977,7 @@ extern "C" int pxb_mx_edge_grad(int64_t cap, const int32_t *from_id, const int32
                                 int32_t batch, int32_t num_units, float *dw, float *weight, const pxb_optimizer *opt,
                                 float *opt_m, float *opt_v, float *opt_t, void *scratch, size_t scratch_bytes,
                                 void *stream) {
-  PXB_REQUIRE(cap >= 0 && batch >= 1 && num_units >= 0, "pxb_mx_edge_grad: bad sizes");
+  PXB_REQUIRE(cap >= 0 && batch >= 1 && batch <= kMxMaxBatch && num_units >= 0, "pxb_mx_edge_grad: bad sizes");
   PXB_REQUIRE(fmt == PXB_MX_E4M3 || fmt == PXB_MX_E5M2, "pxb_mx_edge_grad: a checkpoint has 8 bits (e4m3 or e5m2)");
   if (cap == 0) return PXB_OK;
   PXB_REQUIRE((opt == nullptr) == (dw != nullptr), "pxb_mx_edge_grad: give dw or an optimizer, not both or neither");
@@ -997,7 +997,9 @@ extern "C" int pxb_mx_edge_grad(int64_t cap, const int32_t *from_id, const int32
                    static_cast<int32_t>(mx_blocks(batch)), static_cast<uint32_t>(num_units), dw, weight, op, opt_m,
                    opt_v, opt_t};
   cudaStream_t st = as_stream(stream);
-  const bool wide = !vec || static_cast<int64_t>(num_units) * batch * 4 >= (int64_t(1) << 32);
+  // 32-bit offsets hold the gradients' bytes and the codes' (32 a unit at least: more than the gradients' at few samples)
+  const int64_t row_bytes = batch > mx_blocks(batch) * 8 ? int64_t(batch) * 4 : mx_blocks(batch) * 32;
+  const bool wide = !vec || num_units * row_bytes >= (int64_t(1) << 32);
   if (scratch != nullptr) {
     const size_t need = pair_scratch(cap, batch, num_units);
     if (scratch_bytes < need) {
@@ -1031,17 +1033,18 @@ extern "C" int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src, int32_
                               void *stream) {
   PXB_REQUIRE(conns != nullptr, "pxb_mx_product: conns is NULL");
   PXB_REQUIRE(num_src >= 0 && num_out >= 0 && batch >= 0 && conns->num_dst >= 0 && conns->num_edges >= 0 &&
-                  conns->num_blocks >= 0, "pxb_mx_product: bad sizes");
+                  conns->num_blocks >= 0 && batch <= kMxMaxBatch, "pxb_mx_product: bad sizes");
   PXB_REQUIRE(x_fmt >= PXB_MX_E4M3 && x_fmt <= PXB_MX_F32 && out_fmt >= PXB_MX_E4M3 && out_fmt <= PXB_MX_F32 &&
                   conns->fmt >= PXB_MX_E4M3 && conns->fmt <= PXB_MX_F32, "pxb_mx_product: unknown format");
   PXB_REQUIRE(act_kind >= PXB_ACT_IDENTITY && act_kind <= PXB_ACT_SIGMOID,
               "pxb_mx_product: unknown activation code %d", act_kind);
   if (conns->num_dst == 0 || batch == 0) return PXB_OK;
   PXB_REQUIRE(conns->units && conns->offsets, "pxb_mx_product: a pointer is NULL");
+  PXB_REQUIRE(conns->fmt == PXB_MX_F32 || conns->block_offsets, "pxb_mx_product: block_offsets is NULL");
   if (conns->num_edges > 0) {
     PXB_REQUIRE(conns->src, "pxb_mx_product: a pointer is NULL");
     PXB_REQUIRE(conns->fmt == PXB_MX_F32 ? conns->weight != nullptr
-                                         : conns->block_offsets && (conns->num_blocks == 0 || (conns->codes && conns->scales)),
+                                         : conns->num_blocks == 0 || (conns->codes && conns->scales),
                 "pxb_mx_product: the weights' pointers are NULL");
     PXB_REQUIRE(num_src == 0 || (x_fmt == PXB_MX_F32 ? x != nullptr : x_codes && x_scales),
                 "pxb_mx_product: x is NULL");

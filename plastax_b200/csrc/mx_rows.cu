@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 4) mx_unit_grad_kernel(Grid g, int32
 
 // Rows, blocks a row and the 32-bit block count every launch indexes by.
 static int check_rows(const char *fn, int32_t num_units, int32_t batch, int fmt, int64_t *blocks) {
-  PXB_REQUIRE(num_units >= 0 && batch >= 0, "%s: negative size", fn);
+  PXB_REQUIRE(num_units >= 0 && batch >= 0 && batch <= kMxMaxBatch, "%s: bad size", fn);
   PXB_REQUIRE(mx_format_ok(fmt), "%s: unknown format %d", fn, fmt);
   *blocks = static_cast<int64_t>(num_units) * mx_blocks(batch);
   PXB_REQUIRE(*blocks < (int64_t(1) << 32), "%s: %lld blocks of 32 samples are past 2^32", fn,

@@ -511,6 +511,20 @@ def test_rows_past_four_gigabytes(cuda):
     back = px.mx_dequantize(ck)
     np.testing.assert_array_equal(back[ids].cpu().numpy(), a.astype(np.float32))
     del x, ck, back
+    # few samples: the codes (a whole block a unit) pass 4 GiB long before the gradients do
+    n = (1 << 27) + 64
+    g = torch.zeros((n, 4), device=cuda)
+    rows = px.MxRows.empty(n, 4, "e4m3", cuda, zero=True)
+    ids = torch.tensor([n - 1, 3, n - 33, 64], device=cuda)
+    px.mx_quantize(torch.from_numpy(few[:, :4].copy()).to(cuda), "e4m3", ids=ids, out=rows)
+    g[ids] = torch.from_numpy(few[:, 4:8].copy()).to(cuda)
+    a4 = _mx.values(*_mx.quantize(few[:, :4], "e4m3"), "e4m3", 4)
+    bucket = {"from_id": ids.to(torch.int32), "to_id": ids.flip(0).to(torch.int32),
+              "dead": torch.zeros(4, dtype=torch.uint8, device=cuda)}
+    prod = few[::-1, 4:8].astype(np.float64) * a4
+    out = px.mx_edge_grad(bucket, g, rows).cpu().numpy()
+    assert (np.abs(out - prod.sum(1) / 4) <= 8 * _mx.U32 * np.abs(prod).sum(1) / 4).all()
+    del g, rows
     # 8-bit rows past 4 GiB
     n = (1 << 22) + 4096
     rows = px.MxRows.empty(n, batch, "e4m3", cuda, zero=True)
@@ -821,6 +835,31 @@ def test_captured_and_replayed(cuda):
         for _, outs in graphs:
             for a, b in zip(outs, want):
                 assert torch.equal(a, b)
+
+
+def test_checkpointed_step_captured(cuda):
+    """A captured step replays as the eager one: the same state after each."""
+    rng = np.random.default_rng(31)
+    net, n, frm, to, w, inputs, outputs = _mlp_net([24, 64, 48, 10], 0.3, rng)
+    pair = [px.NetworkBuilder.from_edges(net, n, frm, to, weights=w, input_ids=inputs, output_ids=outputs, device=cuda)
+            for _ in range(2)]
+    steps = [px.make_step(net, static, batch_size=32, device=cuda, activation_checkpoint="e5m2") for static, _ in pair]
+    x, t = torch.zeros((32, 24), device=cuda), torch.zeros((32, 10), device=cuda)
+    run = lambda i: steps[i](pair[i][1], px.StepInputs(x, t))  # noqa: E731
+    run(0), run(1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = run(0)
+    for _ in range(4):
+        x.copy_(torch.randn_like(x)), t.copy_(torch.randn_like(t))
+        graph.replay()
+        want = run(1)
+        # the two forwards and backwards add the same float32 products with atomics: the repository's bar
+        torch.testing.assert_close(res.loss, want.loss, rtol=1e-5, atol=1e-6)
+        for a, b in zip(pair[0][1].conns, pair[1][1].conns):
+            # an activation next to a border of e5m2 may round either way: half a step (2^-3) of one sample's share
+            torch.testing.assert_close(a["weight"], b["weight"], rtol=1e-3, atol=1e-4)
 
 
 def test_two_streams_at_once(cuda):

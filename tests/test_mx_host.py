@@ -163,6 +163,11 @@ def test_abi_refuses_before_a_launch():
     import ctypes
 
     refuse("pxb_mx_product", ctypes.byref(conns), 4, 4, 64, None, None, 3, 0, 4, 64, None, None, 3, None, text="NULL")
+    empty = _lib.MxConns(2, 2, 0, 0, 64, 64, None, None, None, None, None)  # 4-bit weights, no edges, no block offsets
+    refuse("pxb_mx_product", ctypes.byref(empty), 4, 4, 64, None, None, 3, 0, 4, 64, None, None, 3, None,
+           text="block_offsets")
+    refuse("pxb_mx_product", ctypes.byref(conns), 4, (1 << 30) + 1, 64, None, None, 3, 0, 4, 64, None, None, 3, None,
+           text="sizes")
     refuse("pxb_mx_product", None, 4, 4, 64, None, None, 3, 0, 4, 64, None, None, 3, None, text="NULL")
     refuse("pxb_mx_product", ctypes.byref(conns), 4, 4, 64, None, None, 3, 4, 4, 64, None, None, 3, None,
            text="activation")

@@ -802,6 +802,27 @@ def test_infer(cuda, weights, rows, batch):
     _within(got, exact[outputs], exact_err[outputs] + 1e-30)
 
 
+def test_infer_of_a_pruned_net(cuda):
+    """Units left without in-edges (sigmoid of 0, not 0), sources without any
+    (level 0, not an input), and outputs nothing reaches: as the training
+    step's forward."""
+    rng = np.random.default_rng(77)
+    net, n, frm, to, w, inputs, outputs = _mlp_net([16, 30, 20, 6], 0.4, rng, "sigmoid")
+    frm, to = np.append(frm, n).astype(np.int32), np.append(to, 50).astype(np.int32)  # a source that is no input
+    w = np.append(w, np.float32(0.7))
+    static, state = px.NetworkBuilder.from_edges(net, n + 2, frm, to, weights=w, input_ids=inputs,
+                                                 output_ids=[*outputs, n + 1], device=cuda)
+    for b in state.conns:
+        kill = torch.from_numpy(rng.random(b["dead"].numel()) < 0.7).to(cuda) | (b["to_id"] == outputs[0])
+        b["dead"][kill] = 1
+    x = rng.standard_normal((8, len(inputs))).astype(np.float32)
+    got = px.make_infer(net, static, state, weights="f32")(x).cpu().numpy().T
+    step = px.make_step(net, static, batch_size=8, device=cuda)
+    step(state, px.StepInputs(x, np.zeros((8, len(outputs) + 1), np.float32)))
+    np.testing.assert_allclose(got, step.act_b.cpu().numpy()[[*outputs, n + 1]], rtol=1e-5, atol=1e-6)
+    assert not got[0].any() and not got[-1].any()  # identity outputs of nothing
+
+
 def test_captured_and_replayed(cuda):
     """Each operator captured once and replayed on new values in the same
     buffers, two graphs of the same inference sharing nothing."""

@@ -157,7 +157,9 @@ class BatchedStepFn:
         self._check_deeper(state)
         rows.zero_()
         rows.index_copy_(0, inner.input_ids, x.t())
-        mx.mx_quantize(x.t(), ck.fmt, keep_nonzero=True, ids=inner.input_ids, out=ck)
+        # level 0: the inputs' codes, and zeros for the other units there, whose rows in the checkpoint may be another
+        # state's (the levels are the state's, not the step's)
+        mx.mx_unit_apply(rows, ck, "identity", level=level, target_level=0, roles=roles)
         for lv in range(L):
             K.batched_forward(state.conns[lv], rows, rows)
             mx.mx_unit_apply(rows, ck, inner.fwd_act, level=level, target_level=lv + 1, roles=roles)

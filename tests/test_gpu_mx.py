@@ -952,3 +952,45 @@ def test_reads_the_struct_of_the_call(cuda):
     a = px.mx_product(conns, x)
     b = px.mx_product(px.MxConns(conns.units, conns.offsets, conns.src, "f32", weight=conns.weight), x)
     assert torch.equal(a, b)
+
+
+def _levels_net(**kw):
+    class Net(px.Network):
+        forward_pass = px.ForwardPass(kw.get("hidden", "identity"), output_activation="identity")
+        backward_pass = px.BackwardPass(kw.get("hidden", "identity"))
+        loss = px.MSELoss()
+        update_conn = px.optim.sgd(0.5)
+        batch_reduction = px.MeanFloatFirstRest()
+        propagation = px.Propagation.TOPOLOGICAL
+
+    return Net
+
+
+def _built_from(net, n, edges, outputs, dev):
+    frm, to, w = zip(*edges)
+    return px.NetworkBuilder.from_edges(net, n, list(frm), list(to), weights=list(w), input_ids=(0, 1),
+                                        output_ids=outputs, device=dev)
+
+
+@pytest.mark.parametrize("fmt", mx.CHECKPOINT_FORMATS)
+def test_checkpoint_keeps_nothing_of_another_state(cuda, fmt):
+    """Two states of one static, a unit at level 1 in the first and at level 0
+    (without in-edges) in the second: its activation is 0 there, and its
+    out-edges' gradient with it."""
+    net = _levels_net()
+    first = [(0, 2, 1.0), (1, 3, 1.0), (2, 4, 2.0), (3, 4, 1.0)]
+    second = [(1, 3, 1.0), (2, 4, 2.0), (3, 4, 1.0)]
+    static, a = _built_from(net, 5, first, (4,), cuda)
+    static_b, b = _built_from(net, 5, second, (4,), cuda)
+    _, fresh = _built_from(net, 5, second, (4,), cuda)
+    assert static == static_b
+    x, t = np.full((8, 2), 3.0, np.float32), np.zeros((8, 1), np.float32)
+    step = px.make_step(net, static, batch_size=8, device=cuda, activation_checkpoint=fmt)
+    step(a, px.StepInputs(x, t))
+    step(b, px.StepInputs(x, t))
+    px.make_step(net, static, batch_size=8, device=cuda, activation_checkpoint=fmt)(fresh, px.StepInputs(x, t))
+    for mine, want in zip(b.conns, fresh.conns):
+        assert torch.equal(mine["weight"], want["weight"])
+    still = (b.conns[0]["from_id"] == 2) & (b.conns[0]["dead"] == 0)
+    assert b.conns[0]["weight"][still].tolist() == [2.0]
+    assert not px.mx_dequantize(step.checkpoint)[2].any()

@@ -6,11 +6,15 @@ with their weights in MX blocks of 32 in-edges of one unit (or "f32"). The
 returned function runs the forward for a batch of any size, one sample
 included: `infer(inputs)` with inputs (B, num_inputs) gives (B, num_outputs)
 float32, the values the training step's forward leaves in the output units
-(src/plastax/phases.py:972-1015). One kernel a level does the product, the
+(src/plastax/phases.py:972-1015). A unit that the forward never applies (level
+0 and no input, or pruned) keeps its activation: the state's, as the streaming
+step reads it, or 0 for a net with a `batch_reduction`, whose batched step
+starts from rows of zeros. One kernel a level does the product, the
 activation and, with `rows` an MX format, the quantisation of the level's rows
 for the next one; the outputs are always float32.
 
-The layout is a snapshot: later steps on `state` do not change it.
+The layout is a snapshot (of those activations too): later steps on `state` do
+not change it.
 """
 
 from __future__ import annotations
@@ -23,7 +27,7 @@ import torch
 from plastax_b200 import mx
 from plastax_b200.state import NetworkState, NetworkStatic, live_unit_mask
 from plastax_b200.traits import Network
-from plastax_b200.types import LEVEL, Propagation
+from plastax_b200.types import ACTIVATION, LEVEL, Propagation
 
 
 @dataclasses.dataclass(frozen=True)
@@ -77,31 +81,39 @@ class InferFn:
             deeper = (level[t] > level[f]) & ~is_input[t]
             src.append(f[deeper]), dst.append(t[deeper]), w.append(b["weight"][keep][deeper])
         src, dst, w = torch.cat(src), torch.cat(dst), torch.cat(w)
-        # compact rows: the inputs, the level-0 sources (which stay 0), then every other unit that is a source
+        # the units that a level's apply writes; the others keep what they hold
+        applied = live & ~is_input & (level >= 1) & (level <= len(state.conns))
+        held = state.units[ACTIVATION.name].to(torch.float32)
+        if net.batch_reduction is not None:
+            held = torch.zeros_like(held)
+        # compact rows: the inputs, the sources that no apply writes, then every other unit that is a source
         is_source = torch.zeros(n, dtype=torch.bool, device=dev)
         is_source[src] = True
         inputs = torch.tensor(static.input_ids, dtype=torch.int64, device=dev)
-        still = torch.nonzero(is_source & ~is_input & (level == 0)).flatten()
-        moving = torch.nonzero(is_source & ~is_input & (level > 0)).flatten()
+        still = torch.nonzero(is_source & ~is_input & ~applied).flatten()
+        moving = torch.nonzero(is_source & applied).flatten()
         order = torch.cat([inputs, still, moving])
         row_of = torch.full((n,), -1, dtype=torch.int64, device=dev)
         row_of[order] = torch.arange(order.numel(), device=dev)
         self.num_rows, self.num_still = order.numel(), still.numel()
-        self.input_rows = row_of[inputs]
+        self.input_rows, self.still_rows = row_of[inputs], row_of[still]
+        self.still_values = held[still][:, None]
         outputs = torch.tensor(static.output_ids, dtype=torch.int64, device=dev)
         out_of = torch.full((n,), -1, dtype=torch.int64, device=dev)
         out_of[outputs] = torch.arange(outputs.numel(), device=dev)
-        # an output that is an input answers with the input itself; one at level 0 stays 0
+        # an output that is an input answers with the input itself, one that no apply writes with what it holds
         pos = torch.full((n,), -1, dtype=torch.int64, device=dev)
         pos[inputs] = torch.arange(inputs.numel(), device=dev)
         as_input = pos[outputs]
         self.out_from_input = [(i, int(p)) for i, p in enumerate(as_input.tolist()) if p >= 0]
+        self.out_still = torch.nonzero(~is_input[outputs] & ~applied[outputs]).flatten()
+        self.out_still_values = held[outputs[self.out_still]][:, None]
         fp = net.forward_pass
         out_act = fp.output_activation or fp.activation
         rows_src = row_of[src].to(torch.int32)
         self.stages: list[_Stage] = []
-        for lv in range(1, int(level.max().item()) + 1 if n else 1):
-            here = live & (level == lv) & ~is_input
+        for lv in range(1, len(state.conns) + 1):
+            here = applied & (level == lv)
             for sel, act, index, to_outputs in ((here & is_source & ~is_output, fp.activation, row_of, False),
                                                 (here & is_source & is_output, out_act, row_of, False),
                                                 (here & is_output, out_act, out_of, True)):
@@ -129,16 +141,17 @@ class InferFn:
             if self.rows == "f32":
                 rows = torch.empty((self.num_rows, batch), dtype=torch.float32, device=dev)
                 rows[:self.num_inputs] = x.t()
-                rows[self.num_inputs:self.num_inputs + self.num_still] = 0.0
+                rows[self.num_inputs:self.num_inputs + self.num_still] = self.still_values
             else:
                 rows = mx.MxRows.empty(self.num_rows, batch, self.rows, dev)
                 mx.mx_quantize(x.t(), self.rows, ids=self.input_rows, out=rows)
                 if self.num_still:
-                    still = slice(self.num_inputs, self.num_inputs + self.num_still)
-                    rows.codes[still].zero_(), rows.scales[still].zero_()
+                    mx.mx_quantize(self.still_values.expand(-1, batch), self.rows, ids=self.still_rows, out=rows)
             out = torch.zeros((self.num_outputs, batch), dtype=torch.float32, device=dev)
             for s in self.stages:
                 mx.mx_product(s.conns, rows, activation=s.activation, out=out if s.to_outputs else rows)
+            if self.out_still.numel():
+                out.index_copy_(0, self.out_still, self.out_still_values.expand(-1, batch))
             for i, p in self.out_from_input:
                 out[i] = x[:, p]
             return out.t()

@@ -994,3 +994,29 @@ def test_checkpoint_keeps_nothing_of_another_state(cuda, fmt):
     still = (b.conns[0]["from_id"] == 2) & (b.conns[0]["dead"] == 0)
     assert b.conns[0]["weight"][still].tolist() == [2.0]
     assert not px.mx_dequantize(step.checkpoint)[2].any()
+
+
+@pytest.mark.parametrize("rows", ["f32", "e4m3", "e2m1"])
+@pytest.mark.parametrize("batched", [False, True])
+def test_infer_of_units_that_no_level_applies(cuda, rows, batched):
+    """A level-0 unit that is no input keeps the activation its state holds in
+    the streaming step and reads 0 in the batched one; so does an output."""
+    class Net(px.Network):
+        forward_pass = px.ForwardPass("identity")
+        propagation = px.Propagation.TOPOLOGICAL
+        batch_reduction = px.MeanFloatFirstRest() if batched else None
+
+    static, state = _built_from(Net, 6, [(0, 2, 2.0), (3, 2, 4.0), (2, 4, 1.0), (3, 4, -1.0)], (4, 5, 3), cuda)
+    state.units["activation"][3] = 0.5
+    state.units["activation"][5] = 0.25
+    infer = px.make_infer(Net, static, state, weights="f32", rows=rows)
+    for x in ([1.0, 2.0], [-3.0, 0.0]):
+        got = infer(np.array([x] * (8 if batched else 1), np.float32)).cpu().numpy()
+        if batched:
+            step = px.make_step(Net, static, batch_size=8, device=cuda)
+            step(state, px.StepInputs(np.array([x] * 8, np.float32)))
+            want = step.act_b.cpu().numpy()[[4, 5, 3]].T
+        else:
+            px.make_step(Net, static, device=cuda)(state, px.StepInputs(np.array(x, np.float32)))
+            want = state.units["activation"].cpu().numpy()[[4, 5, 3]][None]
+        np.testing.assert_array_equal(got, want)  # few bits: every sum is exact

@@ -235,6 +235,28 @@ def test_infer_layout_is_compact_and_grouped():
         infer(np.zeros((3, 2), np.float32))
 
 
+def test_infer_lays_out_units_that_no_level_applies():
+    """Sources that nothing writes have a row with what the state holds: a
+    pruned unit, a level-0 unit that is no input; a batched net's are 0."""
+    for batched in (False, True):
+        net = _net()
+        if not batched:
+            net.batch_reduction = None
+        static, state = px.NetworkBuilder.from_edges(net, 6, [0, 1, 2, 2, 5, 1], [2, 2, 3, 4, 3, 3], input_ids=(0, 1),
+                                                     output_ids=(3, 4, 5), device="cpu")
+        state.units["pruned"] = torch.tensor([0, 0, 1, 0, 0, 0], dtype=torch.uint8)
+        state.units["activation"][2], state.units["activation"][5] = -0.5, 2.0
+        infer = px.make_infer(net, static, state, weights="f32")
+        assert infer.num_rows == 4 and infer.num_still == 2
+        assert infer.still_rows.tolist() == [2, 3]  # units 2 and 5, after the inputs
+        want = [0.0, 0.0] if batched else [-0.5, 2.0]
+        assert infer.still_values.flatten().tolist() == want
+        assert [s.conns.units.tolist() for s in infer.stages] == [[0, 1]] * 1
+        assert infer.out_still.tolist() == [2] and infer.out_still_values.flatten().tolist() == want[1:]
+        state.units["activation"].fill_(9.0)  # a snapshot
+        assert infer.still_values.flatten().tolist() == want
+
+
 def test_block_counts():
     assert [mx.num_blocks(b) for b in (0, 1, 32, 33, 256)] == [0, 1, 1, 2, 8]
     assert mx.block_bytes("e2m1") == 16 and mx.block_bytes("e5m2") == 32

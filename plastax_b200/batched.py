@@ -19,8 +19,11 @@ made from them in place and, once the checkpoint has them, the backward's sums
 and gradients: 4 (rows) + 4 (the loss seeds) + 33/32 bytes a unit and sample
 instead of 16. A row serves all of these because an edge of a TOPOLOGICAL net
 goes to a deeper level, so a level's sums are complete before its apply. The
-step checks a state for that when it first sees it, and the growth rule must
-have direction "deeper".
+step checks that on a state's columns when it first sees them, and again once
+they were replaced or edited by torch operations (not through `.data` or
+another alias: such an edit needs a new column); the growth rule must have
+direction "deeper". The check reads the host, so a step is run once on a state
+before it is captured, and a captured step does not repeat it.
 """
 
 from __future__ import annotations
@@ -83,7 +86,7 @@ class BatchedStepFn:
         z = lambda: torch.zeros((n, B), dtype=torch.float32, device=device)  # noqa: E731
         self.acc_b = z()
         self.checkpoint = None  # the activations in 8-bit blocks; rows are then shared (see the module's notes)
-        self._checked_state: weakref.ref | None = None
+        self._checked: dict[tuple[int, ...], list] = {}  # the columns that passed _check_deeper, and their versions
         bp, loss = net.backward_pass, net.loss
         if activation_checkpoint is not None:
             self.checkpoint = mx.MxRows.empty(n, B, activation_checkpoint, device, zero=True)
@@ -136,18 +139,27 @@ class BatchedStepFn:
             self.launches += 1
 
     def _check_deeper(self, state: NetworkState) -> None:
-        """Every live edge goes to a deeper level (once per state; reads the
-        host). Edges into inputs, which sit at level 0, do not."""
-        if self._checked_state is not None and self._checked_state() is state:
-            return
+        """Every live edge goes to a deeper level (reads the host, once per
+        set of columns and version of them; the framework's own growth and
+        prune keep it so). Edges into inputs, which sit at level 0, do not."""
         level = state.units[LEVEL.name]
+        cols = [level, *(b[k] for b in state.conns for k in ("from_id", "to_id", "dead"))]
+        key = tuple(map(id, cols))
+        versions = [-1 if t.is_inference() else t._version for t in cols]
+        seen = self._checked.get(key)
+        if seen is not None and all(ref() is t and v == now for (ref, v), t, now in zip(seen, cols, versions)):
+            return
+        if self.dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("activation_checkpoint: the state's edges have not been checked since they were made or "
+                               "edited, and a capture cannot read them: run the step once before capturing it")
         n = self.static.num_units
         for i, b in enumerate(state.conns):
             live = b["dead"] == 0
             f, t = b["from_id"][live].clamp(0, n - 1).long(), b["to_id"][live].clamp(0, n - 1).long()
             if bool((level[t] <= level[f]).any()):
                 raise ValueError(f"activation_checkpoint: bucket {i} has an edge that does not go to a deeper level")
-        self._checked_state = weakref.ref(state)
+        self._checked = {k: v for k, v in self._checked.items() if all(ref() is not None for ref, _ in v)}
+        self._checked[key] = [(weakref.ref(t), v) for t, v in zip(cols, versions)]
 
     def _call_checkpointed(self, state: NetworkState, x: torch.Tensor, inputs: StepInputs) -> None:
         """The propagation and the update of a step whose backward reads the

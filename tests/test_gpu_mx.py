@@ -1020,3 +1020,39 @@ def test_infer_of_units_that_no_level_applies(cuda, rows, batched):
             px.make_step(Net, static, device=cuda)(state, px.StepInputs(np.array(x, np.float32)))
             want = state.units["activation"].cpu().numpy()[[4, 5, 3]][None]
         np.testing.assert_array_equal(got, want)  # few bits: every sum is exact
+
+
+def test_checkpointed_step_knows_its_states(cuda):
+    """Training on two states in turn, with growth and prune, looks at neither
+    again (a capture could not); an edit in place is seen."""
+    rng = np.random.default_rng(21)
+    net, n, frm, to, w, inputs, outputs = _mlp_net([24, 64, 48, 10], 0.3, rng)
+
+    class Grown(net):
+        prune_conn = px.MagnitudePrune(0.02)
+        add_conn = px.ProposeAddConn(proposals_per_proposer=2, max_new_per_level=20, direction="deeper",
+                                     max_level_gap=2, init=("hash_uniform", 0.1))
+
+    built = [px.NetworkBuilder.from_edges(Grown, n, frm, to, weights=w, input_ids=inputs, output_ids=outputs,
+                                          capacity_headroom=0.5, device=cuda) for _ in range(2)]
+    static, states = built[0][0], [s for _, s in built]
+    step = px.make_step(Grown, static, batch_size=32, device=cuda, activation_checkpoint="e4m3")
+    x, t = torch.randn((32, 24), device=cuda), torch.randn((32, 10), device=cuda)
+    for _ in range(3):
+        for s in states:
+            step(s, px.StepInputs(x, t))
+    known = dict(step._checked)
+    for s in states:
+        step(s, px.StepInputs(x, t))
+    assert step._checked == known and len(known) == 2
+    graph = torch.cuda.CUDAGraph()
+    fixed = px.make_step(net, static, batch_size=32, device=cuda, activation_checkpoint="e4m3")
+    fixed(states[0], px.StepInputs(x, t)), fixed(states[1], px.StepInputs(x, t))
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        fixed(states[0], px.StepInputs(x, t))  # not the state seen last
+    graph.replay()
+    torch.cuda.synchronize()
+    states[0].units["level"][outputs[0]] = 1
+    with pytest.raises(ValueError, match="deeper"):
+        step(states[0], px.StepInputs(x, t))

@@ -204,6 +204,37 @@ def test_make_step_refuses_checkpoints_it_cannot_run():
         px.make_step(grown, static, batch_size=8, activation_checkpoint="e4m3", device="cpu")
 
 
+def test_checkpointed_step_checks_edited_columns_again():
+    """The check of a state's edges holds for its columns as they were: edited
+    in place or replaced, they are looked at again; several states stay known."""
+    net = _net()
+    static, a = _built(net)
+    _, b = _built(net)
+    step = px.make_step(net, static, batch_size=8, device="cpu", activation_checkpoint="e4m3")
+    step._check_deeper(a), step._check_deeper(b)
+    known = dict(step._checked)
+    step._check_deeper(a), step._check_deeper(b)
+    assert step._checked == known and len(known) == 2  # nothing was read again
+    a.units["level"][2] = 2  # the same state, a level edited in place: 2 -> 3 and 2 -> 4 stay on a level
+    with pytest.raises(ValueError, match="deeper"):
+        step._check_deeper(a)
+    a.units["level"][2] = 1
+    step._check_deeper(a)
+    a.conns[0]["to_id"][0] = 1
+    with pytest.raises(ValueError, match="deeper"):
+        step._check_deeper(a)
+    a.conns[0]["dead"][0] = 1
+    step._check_deeper(a)
+    cols = dict(b.conns[1])
+    cols["to_id"] = torch.zeros_like(cols["to_id"])
+    b.conns = (b.conns[0], cols)
+    with pytest.raises(ValueError, match="deeper"):
+        step._check_deeper(b)
+    del a, b, cols
+    step._check_deeper(_built(net)[1])
+    assert len(step._checked) == 1  # what is gone is forgotten
+
+
 def test_make_infer_refuses():
     net = _net()
     static, state = _built(net)

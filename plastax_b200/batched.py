@@ -154,8 +154,9 @@ class BatchedStepFn:
                                "edited, and a capture cannot read them: run the step once before capturing it")
         n = self.static.num_units
         for i, b in enumerate(state.conns):
-            live = b["dead"] == 0
-            f, t = b["from_id"][live].clamp(0, n - 1).long(), b["to_id"][live].clamp(0, n - 1).long()
+            f, t = b["from_id"].long(), b["to_id"].long()
+            live = (b["dead"] == 0) & (f >= 0) & (f < n) & (t >= 0) & (t < n)  # as the kernels take them
+            f, t = f[live], t[live]
             if bool((level[t] <= level[f]).any()):
                 raise ValueError(f"activation_checkpoint: bucket {i} has an edge that does not go to a deeper level")
         self._checked = {k: v for k, v in self._checked.items() if all(ref() is not None for ref, _ in v)}

@@ -235,6 +235,15 @@ def test_checkpointed_step_checks_edited_columns_again():
     assert len(step._checked) == 1  # what is gone is forgotten
 
 
+def test_checkpointed_step_does_not_check_edges_out_of_range():
+    """A live slot whose ids are out of range is no edge to the kernels."""
+    net = _net()
+    for column, bad in (("to_id", -1), ("to_id", 5), ("from_id", 5), ("from_id", -(1 << 31))):
+        static, state = _built(net)
+        state.conns[1][column][0] = bad
+        px.make_step(net, static, batch_size=8, device="cpu", activation_checkpoint="e4m3")._check_deeper(state)
+
+
 def test_make_infer_refuses():
     net = _net()
     static, state = _built(net)

@@ -18,8 +18,8 @@ float32 buffer then holds, row by row, the forward's sums, the activations
 made from them in place and, once the checkpoint has them, the backward's sums
 and gradients: 4 (rows) + 4 (the loss seeds) + 33/32 bytes a unit and sample
 instead of 16. A row serves all of these because an edge of a TOPOLOGICAL net
-goes to a deeper level, so a level's sums are complete before its apply. The
-step checks that on a state's columns when it first sees them, and again once
+goes to a deeper level and lies in the bucket of its source's level, so a
+level's sums are complete before its apply. The step checks that on a state's columns when it first sees them, and again once
 they were replaced or edited by torch operations (not through `.data` or
 another alias: such an edit needs a new column); the growth rule must have
 direction "deeper". The check reads the host, so a step is run once on a state
@@ -139,9 +139,10 @@ class BatchedStepFn:
             self.launches += 1
 
     def _check_deeper(self, state: NetworkState) -> None:
-        """Every live edge goes to a deeper level (reads the host, once per
-        set of columns and version of them; the framework's own growth and
-        prune keep it so). Edges into inputs, which sit at level 0, do not."""
+        """Every live edge lies in the bucket of its source's level, whose rows
+        are final when it is swept, and goes to a deeper level (reads the host,
+        once per set of columns and version of them; the framework's own growth
+        and prune keep it so). Edges into inputs, which sit at level 0, do not."""
         level = state.units[LEVEL.name]
         cols = [level, *(b[k] for b in state.conns for k in ("from_id", "to_id", "dead"))]
         key = tuple(map(id, cols))
@@ -157,8 +158,12 @@ class BatchedStepFn:
             f, t = b["from_id"].long(), b["to_id"].long()
             live = (b["dead"] == 0) & (f >= 0) & (f < n) & (t >= 0) & (t < n)  # as the kernels take them
             f, t = f[live], t[live]
-            if bool((level[t] <= level[f]).any()):
+            bad, moved = (level[t] <= level[f]).any(), (level[f] != i).any()
+            if bool(bad):
                 raise ValueError(f"activation_checkpoint: bucket {i} has an edge that does not go to a deeper level")
+            if bool(moved):
+                raise ValueError(f"activation_checkpoint: bucket {i} has an edge whose source is not at level {i}: "
+                                 "resort the state")
         self._checked = {k: v for k, v in self._checked.items() if all(ref() is not None for ref, _ in v)}
         self._checked[key] = [(weakref.ref(t), v) for t, v in zip(cols, versions)]
 

@@ -244,6 +244,19 @@ def test_checkpointed_step_does_not_check_edges_out_of_range():
         px.make_step(net, static, batch_size=8, device="cpu", activation_checkpoint="e4m3")._check_deeper(state)
 
 
+def test_checkpointed_step_refuses_sources_of_another_level():
+    """Bucket i is swept when level i is final: a source that a caller moved to
+    a deeper level, still below its destinations, is read too early."""
+    net = _net()
+    static, state = px.NetworkBuilder.from_edges(net, 6, [0, 1, 2, 5, 5], [2, 5, 5, 3, 4], input_ids=(0, 1),
+                                                 output_ids=(3, 4), device="cpu")
+    step = px.make_step(net, static, batch_size=8, device="cpu", activation_checkpoint="e4m3")
+    step._check_deeper(state)
+    state.conns[0]["from_id"][1], state.conns[0]["to_id"][1] = 2, 3  # 2 -> 3 in the inputs' bucket
+    with pytest.raises(ValueError, match="not at level 0"):
+        step._check_deeper(state)
+
+
 def test_make_infer_refuses():
     net = _net()
     static, state = _built(net)

@@ -282,15 +282,21 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return same_bits<uint32_t>(__floats2bfloat162_rn(lo, hi));
 }
 
-// Two gradients as their three bfloat16 parts (one that is not finite stands in
-// the first part alone).
+__device__ __forceinline__ __nv_bfloat162 cut_bf16(float x, float y) {
+  return __halves2bfloat162(__float2bfloat16_rz(x), __float2bfloat16_rz(y));
+}
+
+// Two gradients as their three bfloat16 parts. The first two are rounded toward
+// zero: 8 + 8 + 8 bits hold a float32 all the same, and the largest float32
+// values, which would round up to infinity, stay finite. One that is not finite
+// stands in the first part alone.
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&p)[3]) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const __nv_bfloat162 h = cut_bf16(x, y);
   const float2 hf = __bfloat1622float2(h);
   float rx = __fsub_rn(x, hf.x), ry = __fsub_rn(y, hf.y);
   if (!isfinite(hf.x)) rx = 0.0f;
   if (!isfinite(hf.y)) ry = 0.0f;
-  const __nv_bfloat162 m = __floats2bfloat162_rn(rx, ry);
+  const __nv_bfloat162 m = cut_bf16(rx, ry);
   const float2 mf = __bfloat1622float2(m);
   p[0] = same_bits<uint32_t>(h);
   p[1] = same_bits<uint32_t>(m);

@@ -1056,3 +1056,26 @@ def test_checkpointed_step_knows_its_states(cuda):
     states[0].units["level"][outputs[0]] = 1
     with pytest.raises(ValueError, match="deeper"):
         step(states[0], px.StepInputs(x, t))
+
+
+@pytest.mark.parametrize("fmt", mx.CHECKPOINT_FORMATS)
+def test_edge_grad_of_the_largest_gradients(cuda, fmt):
+    """Gradients up to float32's largest against small activations, slot by
+    slot and as one product: sums that float32 holds stay finite."""
+    rng = np.random.default_rng(11)
+    n, batch = 70, 256
+    g = (rng.standard_normal((n, batch)) * np.exp2(rng.integers(-40, 90, (n, 1)))).astype(np.float32)
+    big = np.finfo(np.float32).max
+    g[::3, ::7] = big * rng.choice([1.0, -1.0, 1 - 2.0 ** -9, 1 - 2.0 ** -16], g[::3, ::7].shape)
+    x = (rng.standard_normal((n, batch)) * 2.0 ** -12).astype(np.float32)
+    x[:, 5:9] = 0.0
+    ck = _rows(x, fmt, True, cuda)
+    a = _mx.values(ck.codes.cpu().numpy(), ck.scales.cpu().numpy(), fmt, batch)
+    for cap in (1000, 1 << 18):
+        assert (mx.edge_grad_scratch_bytes(cap, batch, n) > 0) == (cap > 1000)
+        f, t = rng.integers(0, n, cap).astype(np.int32), rng.integers(0, n, cap).astype(np.int32)
+        dev = {"from_id": torch.from_numpy(f).to(cuda), "to_id": torch.from_numpy(t).to(cuda),
+               "dead": torch.zeros(cap, dtype=torch.uint8, device=cuda)}
+        pairs, size = g.astype(np.float64) @ a.T / batch, np.abs(g).astype(np.float64) @ np.abs(a).T / batch
+        got = px.mx_edge_grad(dev, torch.from_numpy(g).to(cuda), ck).cpu().numpy()
+        _within(got, pairs[t, f], size[t, f] * (batch + 4) * _mx.U32 * 1.01, f"{cap} slots")

@@ -403,7 +403,9 @@ typedef struct pxb_mx_conns {
  * as they were. x is float32 [num_src, B] or MX rows; out float32 [num_out, B]
  * or MX rows (quantised from the float32 result). An edge whose source is
  * outside [0, num_src) and a unit outside [0, num_out) are skipped. x and out
- * may be one buffer where no destination is a source. */
+ * may be one buffer where no destination is a source. A weight times a block's
+ * scale is formed first: where that is below 2^-126 it keeps a subnormal's
+ * bits, 2^-150 of absolute error before the code's factor. */
 PXB_API int pxb_mx_product(const pxb_mx_conns *conns, int32_t num_src,
                            int32_t batch, const float *x,
                            const uint8_t *x_codes, const uint8_t *x_scales,

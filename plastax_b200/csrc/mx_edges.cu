@@ -633,7 +633,7 @@ __device__ __forceinline__ Piece<XF> load_piece(const Rows &r, O row, float w, b
     constexpr int kShift = XF == PXB_MX_E2M1 ? 4 : 5;  // a block's bytes of codes
     p.v = __ldg(reinterpret_cast<const uint4 *>(r.codes + row) + piece);
     const uint32_t s = __ldg(r.scales + (row >> kShift) + (piece >> (kShift - 4)));
-    // as mx_scale_value, but for 255: infinite, which the block's codes, 0, make not a number
+    // as mx_scale_value, but for 255: infinite, so that the sums are not finite and sum_scaled takes the item
     const float f = __fmul_rn(w, __uint_as_float(max(s << 23, 0x00400000u)));
     p.w = valid ? f : 0.0f;
     if (XF != PXB_MX_E2M1 && !valid) p.v = make_uint4(0, 0, 0, 0);
@@ -657,6 +657,48 @@ __device__ __forceinline__ void add_piece(const Piece<XF> &p, float2 (&acc)[Piec
       mx_decode_word<XF>(v[i], h);
 #pragma unroll
       for (int q = 0; q < kPairs; ++q) acc[i * kPairs + q] = ffma2(w, __half22float2(h[q]), acc[i * kPairs + q]);
+    }
+  }
+}
+
+// An item's sums again, each value with its scale before the weight, as a
+// float32 row would hold it: for where weight times scale left float32's range
+// though products with the block's small values do not (or a block is not a
+// number). add_piece then had an infinite factor, which leaves every sum of its
+// piece infinite or not a number, so one look at one sum an item finds it.
+// (The order does not matter otherwise: a power of two, and one rounding.)
+template <int XF, int LANES, typename O>
+__device__ __forceinline__ void sum_scaled(const Conns &c, const Rows &r, const Item &it, int32_t first, int32_t step,
+                                           int32_t piece, O row_bytes, float2 (&acc)[Piece<XF>::kSamples / 2]) {
+  constexpr int kShift = XF == PXB_MX_E2M1 ? 4 : 5, kPairs = 32 / (2 * MxFormat<XF>::bits), kGroups = 32 / LANES;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int q = 0; q < Piece<XF>::kSamples / 2; ++q) acc[q] = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+  for (int32_t k = first; k < it.blocks; k += step) {
+    int32_t src;
+    float weight;
+    load_edge(c, it, k, lane, r.rows, src, weight);
+#pragma unroll 1
+    for (int j = 0; j < 32; j += kGroups) {
+      const int32_t f = __shfl_sync(0xffffffffu, src, j + lane / LANES);
+      const float w = __shfl_sync(0xffffffffu, weight, j + lane / LANES);
+      if (f < 0) continue;
+      const O row = static_cast<O>(f) * row_bytes;
+      const uint4 codes = __ldg(reinterpret_cast<const uint4 *>(r.codes + row) + piece);
+      const float s = mx_scale_value(__ldg(r.scales + (row >> kShift) + (piece >> (kShift - 4))));
+      const uint32_t v[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __half2 h[kPairs];
+        mx_decode_word<XF>(v[i], h);
+#pragma unroll
+        for (int q = 0; q < kPairs; ++q) {
+          const float2 x = __half22float2(h[q]);
+          acc[i * kPairs + q] = ffma2(make_float2(w, w), make_float2(__fmul_rn(x.x, s), __fmul_rn(x.y, s)),
+                                      acc[i * kPairs + q]);
+        }
+      }
     }
   }
 }
@@ -727,6 +769,10 @@ __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int
 #pragma unroll
           for (int d = 0; d < kDepth; ++d) add_piece<XF>(p[d], acc);
         }
+      }
+      if constexpr (XF != PXB_MX_F32) {
+        if (__any_sync(0xffffffffu, !(fabsf(acc[0].x) < INFINITY)))
+          sum_scaled<XF, LANES, O>(c, r, it, member + rank * n.wpd, step, piece, row_bytes, acc);
       }
     }
     // the edges read side by side join

@@ -1079,3 +1079,49 @@ def test_edge_grad_of_the_largest_gradients(cuda, fmt):
         pairs, size = g.astype(np.float64) @ a.T / batch, np.abs(g).astype(np.float64) @ np.abs(a).T / batch
         got = px.mx_edge_grad(dev, torch.from_numpy(g).to(cuda), ck).cpu().numpy()
         _within(got, pairs[t, f], size[t, f] * (batch + 4) * _mx.U32 * 1.01, f"{cap} slots")
+
+
+@pytest.mark.parametrize("rows", FMTS)
+@pytest.mark.parametrize("weights", ["e2m1", "f32"])
+@pytest.mark.parametrize("degrees,batch", [("one", 7), ("one", 20), ("ragged", 33), ("ragged", 64), ("ragged", 100),
+                                           ("long", 250), ("single", 20), ("single", 300)])
+def test_product_of_large_rows_and_weights(cuda, rows, weights, degrees, batch):
+    """Weights whose product with a block's scale passes float32's range: every
+    sample whose own products stay in it is as in float32, a 0 among them."""
+    rng = np.random.default_rng(batch)
+    num_src = 12
+    degrees = {**DEGREES, "single": [1] * 40}[degrees]
+    conns, off, src, w, units = _graph(rng, degrees, num_src, "f32", cuda)
+    w = (np.sign(w) * np.exp2(rng.integers(-20, 40, w.size)) * rng.choice([1.0, 1.5], w.size)).astype(np.float32)
+    w[0] = 1.5 * 2.0 ** 39
+    if weights == "f32":
+        conns = px.MxConns(conns.units, conns.offsets, conns.src, "f32", weight=torch.from_numpy(w).to(cuda))
+    else:
+        deg = np.asarray(degrees)
+        dst = torch.from_numpy(np.repeat(np.arange(deg.size), deg)).to(cuda)
+        made = px.MxConns.from_edges(conns.src, dst, torch.from_numpy(w).to(cuda),
+                                     torch.arange(deg.size, dtype=torch.int32, device=cuda), weights=weights)
+        conns = px.MxConns(conns.units, made.offsets, made.src, weights, block_offsets=made.block_offsets,
+                           codes=made.codes, scales=made.scales)
+        v = _mx.values(made.codes.cpu().numpy(), made.scales.cpu().numpy()[:, None], weights, 32).reshape(-1)
+        blk = made.block_offsets.cpu().numpy()
+        w = np.concatenate([v[blk[i] * 32:blk[i] * 32 + deg[i]] for i in range(deg.size)])
+    x = rng.standard_normal((num_src, batch)) * np.exp2(rng.integers(-30, 20, (num_src, batch)))
+    x[:, ::5] = 0.0
+    x[:, 3::11] *= 2.0 ** 100  # a few samples of a block, whose scale then is large
+    x[src[0], 3] = 2.0 ** 120
+    x = x.astype(np.float32)
+    xd = _rows(x, rows, False, cuda)
+    xv = _mx.values(xd.codes.cpu().numpy(), xd.scales.cpu().numpy(), rows, batch)
+    total = len(units) + 4
+    got = px.mx_product(conns, xd, out=torch.zeros((total, batch), device=cuda)).cpu().numpy()
+    y, err = _mx.product(off, src, w, xv, units, total, "identity", num_src)
+    top = np.zeros((total, batch))
+    for i, u in enumerate(units):
+        e = np.arange(off[i], off[i + 1])
+        if e.size:
+            top[u] = np.abs(w[e, None] * xv[src[e]]).sum(0)
+    fits = top < 2.0 ** 126
+    assert fits.any() and not fits[units].all()
+    _within(got[fits], y[fits], err[fits])
+    assert not np.isfinite(got[(top > 2.0 ** 129) & (np.abs(y) > 2.0 ** 128.5)]).any()

@@ -346,7 +346,8 @@ PXB_API int pxb_mx_dequantize(int32_t num_units, int32_t batch,
  * for the units with level == target_level (level NULL: all), rows = act(rows)
  * in place (a unit of role 1 keeps its row) and the result's codes with
  * keep_nonzero, e4m3 or e5m2. Replaces pxb_batched_unit_apply mode 0 when the
- * backward reads a checkpoint. */
+ * backward reads a checkpoint; unlike it, a ReLU keeps what is not a number
+ * (so does pxb_mx_product's; its derivative there is 0, as everywhere). */
 PXB_API int pxb_mx_unit_apply(int32_t num_units, int32_t batch,
                               int32_t act_kind, float *rows,
                               const int32_t *level, int32_t target_level,

@@ -13,7 +13,8 @@ growth run once on the reduced state, as the streaming step runs them.
 
 With `activation_checkpoint` ("e4m3" / "e5m2", plastax_b200/mx.py) the backward
 pass and the update read the activations from 8-bit blocks that the forward's
-applies leave behind; the forward and the loss stay in float32. One [N, B]
+applies leave behind; the forward and the loss stay in float32 (a ReLU keeps
+what is not a number, which the plain step's makes 0). One [N, B]
 float32 buffer then holds, row by row, the forward's sums, the activations
 made from them in place and, once the checkpoint has them, the backward's sums
 and gradients: 4 (rows) + 4 (the loss seeds) + 33/32 bytes a unit and sample

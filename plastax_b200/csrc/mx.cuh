@@ -193,6 +193,12 @@ __device__ __forceinline__ uint32_t mx_amax8(const float (&x)[8]) {
   return m;
 }
 
+// A unit's activation. A ReLU keeps what is not a number (act_fn's comparison
+// makes it 0): a poisoned block must not read as a silent unit.
+__device__ __forceinline__ float mx_act(int kind, float x) {
+  return kind == PXB_ACT_RELU ? (x <= 0.0f ? 0.0f : x) : act_fn(kind, x);
+}
+
 // Division by a launch constant: n / d for n < 2^32 as a multiply-high
 // (round-up method; exact for every 32-bit n with a 33-bit magic number).
 struct FastDiv {

@@ -529,7 +529,7 @@ __device__ __forceinline__ void finish_octet(const Conns &c, const Rows &r, int 
     b = static_cast<int32_t>(item - i * n.chunks.d) * CHUNK + o;
     sum(v);
 #pragma unroll
-    for (int z = 0; z < 8; ++z) v[z] = b + z < r.batch ? act_fn(act_kind, v[z]) : 0.0f;
+    for (int z = 0; z < 8; ++z) v[z] = b + z < r.batch ? mx_act(act_kind, v[z]) : 0.0f;
   }
   const bool on = live && b < r.nb * kMxBlock && static_cast<uint32_t>(u) < out.rows;
   if (out.fmt == PXB_MX_F32) {
@@ -868,7 +868,7 @@ __global__ void __launch_bounds__(256) mx_product_short_kernel(Conns c, Rows r, 
       fold_lanes<4, 1, N>(f, lane, base);
 #pragma unroll
       for (int z = 0; z < (N > 8 ? N / 8 : 1); ++z)
-        if (on && base + z < r.batch) out.x[static_cast<int64_t>(u) * r.batch + base + z] = act_fn(act_kind, f[z]);
+        if (on && base + z < r.batch) out.x[static_cast<int64_t>(u) * r.batch + base + z] = mx_act(act_kind, f[z]);
       continue;
     }
 #pragma unroll
@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(256) mx_product_short_kernel(Conns c, Rows r, 
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < N; ++b) {
-      const float y = b < r.batch ? act_fn(act_kind, f[b]) : 0.0f;
+      const float y = b < r.batch ? mx_act(act_kind, f[b]) : 0.0f;
       m = max(m, __float_as_uint(y) & 0x7fffffffu);
       if (sub == b / 8) v[b % 8] = y;
     }

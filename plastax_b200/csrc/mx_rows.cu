@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kThreads) mx_unit_apply_kernel(Grid g, int32_t
       if (role != 1) {
         const int kind = unit_act_kind(act_kind, role);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = o.b + i < g.batch ? act_fn(kind, v[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = o.b + i < g.batch ? mx_act(kind, v[i]) : 0.0f;
       }
     }
     put<float, LAYOUT>(g, static_cast<uint32_t>(t), o, rows, g.batch, moves, buf, v);

@@ -222,7 +222,9 @@ def mx_unit_apply(rows: torch.Tensor, checkpoint: MxRows, activation, *, level: 
                   target_level: int = 0, roles: torch.Tensor | None = None) -> None:
     """rows = activation(rows) in place for the units at `target_level` (all,
     without `level`; an input, role 1, keeps its row), and their checkpoint
-    with `keep_nonzero`. `activation`: a name, or (name, the outputs' name)."""
+    with `keep_nonzero`. `activation`: a name, or (name, the outputs' name). A
+    ReLU keeps what is not a number (the float32 step's makes it 0), so a
+    poisoned row does not read as a silent one."""
     n, b = _rows_shape(rows, "mx_unit_apply: rows")
     _format(checkpoint.fmt, CHECKPOINT_FORMATS, "checkpoint format")
     _tensor(rows, torch.float32, (checkpoint.num_units, checkpoint.batch), "mx_unit_apply: rows", checkpoint.device)
@@ -388,7 +390,8 @@ class MxConns:
 def mx_product(conns: MxConns, x: torch.Tensor | MxRows, *, activation: str = "identity",
                out: torch.Tensor | MxRows | None = None) -> torch.Tensor | MxRows:
     """out[units[i], b] = activation(sum_e w[e] * x[src[e], b]), summed in
-    float32; activation(0) for a destination without edges.
+    float32; activation(0) for a destination without edges. A ReLU keeps what is
+    not a number.
 
     x: float32 rows [num_units, batch] or MX rows. `out`: float32 rows or MX
     rows of the same batch, written at the destinations' rows only (a new

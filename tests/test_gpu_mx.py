@@ -1125,3 +1125,44 @@ def test_product_of_large_rows_and_weights(cuda, rows, weights, degrees, batch):
     assert fits.any() and not fits[units].all()
     _within(got[fits], y[fits], err[fits])
     assert not np.isfinite(got[(top > 2.0 ** 129) & (np.abs(y) > 2.0 ** 128.5)]).any()
+
+
+def test_relu_keeps_what_is_not_a_number(cuda):
+    rng = np.random.default_rng(4)
+    for many, batch in ((700, 40), (11000, 1), (11000, 8), (11000, 16), (3, 300)):
+        conns, off, src, w, units = _graph(rng, [5] * many, 16, "f32", cuda)
+        x = rng.standard_normal((16, batch)).astype(np.float32)
+        x[src[0], batch // 2] = np.nan
+        x[src[7], 0] = np.inf
+        xf = torch.from_numpy(x).to(cuda)
+        total = len(units) + 3
+        for xd in (xf, *(px.mx_quantize(xf, fmt) for fmt in FMTS)):
+            ident = px.mx_product(conns, xd, out=torch.zeros((total, batch), device=cuda))
+            relu = px.mx_product(conns, xd, activation="relu", out=torch.zeros((total, batch), device=cuda))
+            assert torch.isnan(ident).any()
+            assert torch.equal(torch.isnan(relu), torch.isnan(ident))
+            assert torch.equal(torch.nan_to_num(relu, 0.0), torch.clamp_min(torch.nan_to_num(ident, 0.0), 0.0))
+            for fmt in FMTS:
+                q = px.mx_product(conns, xd, activation="relu", out=px.MxRows.empty(total, batch, fmt, cuda, zero=True))
+                bad = torch.nn.functional.pad(~torch.isfinite(relu), (0, -batch % 32)).view(total, -1, 32).any(2)
+                assert torch.equal(q.scales == 255, bad)
+
+
+@pytest.mark.parametrize("fmt", mx.CHECKPOINT_FORMATS)
+def test_relu_apply_keeps_what_is_not_a_number(cuda, fmt):
+    rows = torch.randn((20, 70), device=cuda)
+    rows[3, 40], rows[7, 2] = float("nan"), float("inf")
+    want = torch.relu(rows)
+    ck = px.MxRows.empty(20, 70, fmt, cuda)
+    px.mx_unit_apply(rows, ck, "relu")
+    assert torch.equal(torch.isnan(rows), torch.isnan(want)) and torch.equal(torch.nan_to_num(rows), torch.nan_to_num(want))
+    bad = torch.zeros((20, 3), dtype=torch.bool, device=cuda)
+    bad[3, 1] = bad[7, 0] = True
+    assert torch.equal(ck.scales == 255, bad)
+    net, n, frm, to, w, inputs, outputs = _mlp_net([24, 40, 33, 10], 0.4, np.random.default_rng(1))
+    static, state = px.NetworkBuilder.from_edges(net, n, frm, to, weights=w, input_ids=inputs, output_ids=outputs, device=cuda)
+    x = np.random.default_rng(2).standard_normal((40, 24)).astype(np.float32)
+    x[33, 5] = np.nan
+    for r, first in (("f32", 33), ("e4m3", 32)):
+        got = torch.isnan(px.make_infer(net, static, state, weights="f32", rows=r)(x))
+        assert got[first:].any() and not got[:first].any() and (r != "f32" or not got[34:].any())

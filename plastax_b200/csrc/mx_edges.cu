@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(256) mx_edge_grad_split_kernel(EdgeGrad k) {
 // touches are computed; the product lies in the caller's scratch, n^2 floats,
 // in L2. mma.sync is the bound of the middle kernel (tensor pipes 30 % busy over
 // its two rounds of tiles); the launches around it cost as much again.
-constexpr int kPairTile = 64, kPairUnits = 4096;
+constexpr int kPairTile = 64, kPairUnits = 4096, kPairSlots = 49152;
 
 __host__ __device__ inline int pair_tiles(uint32_t n) { return static_cast<int>((n + kPairTile - 1) / kPairTile); }
 
@@ -968,9 +968,13 @@ static int launch_product(const Conns &c, const Rows &r, int act, const Out &out
 // Scratch of the pair product (0 where slot by slot is as good): the pairs'
 // sums, then a bit a tile. At a twelfth of all pairs of units (between two
 // levels of a layered net a third or more of theirs) the two are alike; and
-// enough work to pay for four launches.
+// enough work to pay for four launches. A tile is one CTA over the whole batch,
+// so a small net's long batch is few CTAs' work however many slots it has, and
+// the slots have to be worth that: 64 units, 4,096 samples, slot by slot and so:
+// 32,768 slots 63 and 82 us, 65,536 slots 112 and 83 (16, 128 and 300 units and
+// 1,024 to 16,384 samples: the same border).
 static size_t pair_scratch(int64_t cap, int32_t batch, int64_t n) {
-  if (n > kPairUnits || cap * 12 < n * n || cap * batch < (int64_t(1) << 26)) return 0;
+  if (n > kPairUnits || cap * 12 < n * n || cap * batch < (int64_t(1) << 26) || cap < kPairSlots) return 0;
   const int64_t tiles = pair_tiles(static_cast<uint32_t>(n));
   return static_cast<size_t>(n * n * 4 + (tiles * tiles + 31) / 32 * 4);
 }

@@ -1166,3 +1166,18 @@ def test_relu_apply_keeps_what_is_not_a_number(cuda, fmt):
     for r, first in (("f32", 33), ("e4m3", 32)):
         got = torch.isnan(px.make_infer(net, static, state, weights="f32", rows=r)(x))
         assert got[first:].any() and not got[:first].any() and (r != "f32" or not got[34:].any())
+
+
+@pytest.mark.parametrize("n,cap,batch", [(64, 4096, 16384), (2, 5, 1 << 17), (16, 20000, 5001)])
+def test_edge_grad_of_a_long_batch(cuda, n, cap, batch):
+    rng = np.random.default_rng(batch)
+    b, dev = _bucket(rng, n, cap, cuda)
+    g = rng.standard_normal((n, batch)).astype(np.float32)
+    ck = _rows(rng.standard_normal((n, batch)).astype(np.float32), "e4m3", True, cuda)
+    a = _mx.values(ck.codes.cpu().numpy(), ck.scales.cpu().numpy(), "e4m3", batch)
+    f, t = b["from_id"].astype(np.int64), b["to_id"].astype(np.int64)
+    live = (b["dead"] == 0) & (f >= 0) & (f < n) & (t >= 0) & (t < n)
+    f, t = np.where(live, f, 0), np.where(live, t, 0)
+    pairs, size = g.astype(np.float64) @ a.T / batch, np.abs(g).astype(np.float64) @ np.abs(a).T / batch
+    got = px.mx_edge_grad(dev, torch.from_numpy(g).to(cuda), ck).cpu().numpy()
+    _within(got, np.where(live, pairs[t, f], 0.0), np.where(live, size[t, f] * (batch + 4) * _mx.U32 * 1.01, 0.0))

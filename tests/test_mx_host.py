@@ -310,6 +310,14 @@ def test_infer_lays_out_units_that_no_level_applies():
         assert infer.still_values.flatten().tolist() == want
 
 
+def test_few_slots_of_a_long_batch_go_slot_by_slot():
+    """One product of all pairs gives a tile of units one CTA for the whole
+    batch: a small net's few slots are spread over the batch instead."""
+    for sizes in ((4096, 16384, 64), (32768, 16384, 16), (16384, 1 << 20, 128), (4, 1 << 24, 2)):
+        assert mx.edge_grad_scratch_bytes(*sizes) == 0
+    assert mx.edge_grad_scratch_bytes(65536, 1024, 64) == 64 * 64 * 4 + 4
+
+
 def test_block_counts():
     assert [mx.num_blocks(b) for b in (0, 1, 32, 33, 256)] == [0, 1, 1, 2, 8]
     assert mx.block_bytes("e2m1") == 16 and mx.block_bytes("e5m2") == 32

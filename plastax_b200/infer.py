@@ -76,8 +76,9 @@ class InferFn:
         is_output[list(static.output_ids)] = True
         src, dst, w = [], [], []
         for b in state.conns:
-            keep = b["dead"] == 0
-            f, t = b["from_id"][keep].long(), b["to_id"][keep].long()
+            f, t = b["from_id"].long(), b["to_id"].long()
+            keep = (b["dead"] == 0) & (f >= 0) & (f < n) & (t >= 0) & (t < n)  # as the step's kernels take them
+            f, t = f[keep], t[keep]
             # an edge that is not to a deeper level arrives after its destination's apply
             deeper = (level[t] > level[f]) & ~is_input[t]
             src.append(f[deeper]), dst.append(t[deeper]), w.append(b["weight"][keep][deeper])

@@ -318,6 +318,17 @@ def test_few_slots_of_a_long_batch_go_slot_by_slot():
     assert mx.edge_grad_scratch_bytes(65536, 1024, 64) == 64 * 64 * 4 + 4
 
 
+def test_infer_leaves_out_edges_out_of_range():
+    """A live slot whose ids are out of range is no edge, as in the step (on a
+    GPU, indexing by it would be a device assert)."""
+    net = _net()
+    for column, bad in (("to_id", -1), ("to_id", 5), ("from_id", 5), ("from_id", -2), ("from_id", -(1 << 31))):
+        static, state = _built(net)
+        state.conns[1][column][0] = bad
+        infer = px.make_infer(net, static, state, weights="f32")
+        assert infer.num_edges == 3 and infer.stages[-1].conns.offsets.tolist() == [0, 0, 1]
+
+
 def test_block_counts():
     assert [mx.num_blocks(b) for b in (0, 1, 32, 33, 256)] == [0, 1, 1, 2, 8]
     assert mx.block_bytes("e2m1") == 16 and mx.block_bytes("e5m2") == 32

@@ -40,6 +40,7 @@ CHECKPOINT_FORMATS = ("e4m3", "e5m2")
 WEIGHT_FORMATS = (*FORMATS, "f32")
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MAX_BATCH = 1 << 24
+_MAX_UNITS = (1 << 31) - 1  # the C ABI's counts are 32-bit
 _U8 = torch.uint8
 
 
@@ -103,7 +104,7 @@ def _rows_shape(x: torch.Tensor, what: str) -> tuple[int, int]:
     if len(shape) != 2:
         raise ValueError(f"{what}: expected unit rows [num_units, batch], got shape {tuple(shape)}")
     n, b = shape
-    if n >= 1 << 31 or b > _MAX_BATCH:
+    if n > _MAX_UNITS or b > _MAX_BATCH:
         raise ValueError(f"{what}: [{n}, {b}] is past 2^31 - 1 units or {_MAX_BATCH} samples")
     return n, b
 
@@ -123,6 +124,8 @@ class MxRows:
         _format(self.fmt)
         if not 0 <= self.batch <= _MAX_BATCH:
             raise ValueError(f"MxRows: batch must be in [0, {_MAX_BATCH}], got {self.batch}")
+        if isinstance(scales, torch.Tensor) and scales.dim() == 2 and scales.shape[0] > _MAX_UNITS:
+            raise ValueError(f"MxRows: {scales.shape[0]} units are past 2^31 - 1")
         nb = num_blocks(self.batch)
         if isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype is _U8 and \
                 scales.dtype is _U8 and scales.dim() == 2 and scales.shape[1] == nb and \
@@ -150,6 +153,8 @@ class MxRows:
         _format(fmt)
         if not 0 <= batch <= _MAX_BATCH:
             raise ValueError(f"MxRows: batch must be in [0, {_MAX_BATCH}], got {batch}")
+        if num_units > _MAX_UNITS:
+            raise ValueError(f"MxRows: {num_units} units are past 2^31 - 1")
         new = torch.zeros if zero else torch.empty
         nb = num_blocks(batch)
         rows = object.__new__(cls)  # nothing to check in what is made here
@@ -336,6 +341,8 @@ class MxConns:
         fmt = _format(self.weights, WEIGHT_FORMATS, "weight format")
         units, offsets, src = self.units, self.offsets, self.src
         dev, m, e = units.device, units.numel(), src.numel()
+        if m > _MAX_UNITS:
+            raise ValueError(f"MxConns.units: {m} destinations are past 2^31 - 1")
         _tensor(units, torch.int32, (m,), "MxConns.units")
         _tensor(offsets, torch.int64, (m + 1,), "MxConns.offsets", dev)
         _tensor(src, torch.int32, (e,), "MxConns.src", dev)

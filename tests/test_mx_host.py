@@ -329,6 +329,22 @@ def test_infer_leaves_out_edges_out_of_range():
         assert infer.num_edges == 3 and infer.stages[-1].conns.offsets.tolist() == [0, 0, 1]
 
 
+def test_counts_past_32_bits_are_refused():
+    """The C ABI counts units in 32 bits: more would be cut off without a word."""
+    n = (1 << 31) + 7
+    big = lambda *shape, dtype=torch.uint8: torch.empty(shape, dtype=dtype, device="meta")  # noqa: E731
+    with pytest.raises(ValueError, match="2\\^31"):
+        px.MxRows(big(n, 32), big(n, 1), "e4m3", 1)
+    with pytest.raises(ValueError, match="2\\^31"):
+        px.MxRows.empty(n, 1, "e2m1", "meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        px.mx_quantize(big(n, 1, dtype=torch.float32), "e4m3")
+    with pytest.raises(ValueError, match="2\\^31"):
+        px.MxConns(big(n, dtype=torch.int32), big(n + 1, dtype=torch.int64), big(5, dtype=torch.int32), "f32",
+                   weight=big(5, dtype=torch.float32))
+    assert px.MxRows(big(5, 32), big(5, 1), "e4m3", 1).num_units == 5
+
+
 def test_block_counts():
     assert [mx.num_blocks(b) for b in (0, 1, 32, 33, 256)] == [0, 1, 1, 2, 8]
     assert mx.block_bytes("e2m1") == 16 and mx.block_bytes("e5m2") == 32

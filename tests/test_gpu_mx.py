@@ -1181,3 +1181,67 @@ def test_edge_grad_of_a_long_batch(cuda, n, cap, batch):
     pairs, size = g.astype(np.float64) @ a.T / batch, np.abs(g).astype(np.float64) @ np.abs(a).T / batch
     got = px.mx_edge_grad(dev, torch.from_numpy(g).to(cuda), ck).cpu().numpy()
     _within(got, np.where(live, pairs[t, f], 0.0), np.where(live, size[t, f] * (batch + 4) * _mx.U32 * 1.01, 0.0))
+
+
+def test_checkpointed_step_of_a_small_net_with_many_slots(cuda):
+    """The update as one product of all pairs, reached through the step: one
+    SGD step from the step's own gradient rows and checkpoint, in 64 bits."""
+    rng = np.random.default_rng(41)
+    net, n, frm, to, w, inputs, outputs = _mlp_net([40, 50, 10], 0.5, rng, opt=px.optim.sgd(0.05))
+    static, state = px.NetworkBuilder.from_edges(net, n, frm, to, weights=w, input_ids=inputs, output_ids=outputs,
+                                                 capacity_align=1 << 16, device=cuda)
+    assert all(mx.edge_grad_scratch_bytes(b["dead"].numel(), 1024, n) > 0 for b in state.conns)
+    step = px.make_step(net, static, batch_size=1024, device=cuda, activation_checkpoint="e4m3")
+    before = [{k: b[k].cpu().numpy() for k in ("from_id", "to_id", "dead", "weight")} for b in state.conns]
+    step(state, px.StepInputs(rng.standard_normal((1024, 40)).astype(np.float32),
+                              rng.standard_normal((1024, 10)).astype(np.float32)))
+    g, a = step.grad_b.cpu().numpy(), px.mx_dequantize(step.checkpoint).cpu().numpy().astype(np.float64)
+    for h, b in zip(before, state.conns):
+        live, dw, err = _edge_reference(h, g, a, n)
+        w0 = h["weight"].astype(np.float64)
+        got = b["weight"].cpu().numpy()
+        lr = float(np.float32(0.05))
+        # the gradient's error, then a rounding of lr * dw and one of the difference
+        bound = lr * err + 2 * _mx.U32 * (np.abs(w0) + lr * np.abs(dw)) * 1.01
+        assert live.any() and (np.abs(got - (w0 - lr * dw))[live] <= bound[live]).all()
+        np.testing.assert_array_equal(got[~live], h["weight"][~live])
+
+
+def test_four_bit_answers_after_training(cuda):
+    """A trained net's answers from 4-bit weights: those of its weights as
+    held, off the float32 net's by no more than the weights' rounding carries
+    forward, so that a class it leads by more than that stays the class."""
+    rng = np.random.default_rng(51)
+    net, n, frm, to, w, inputs, outputs = _mlp_net([16, 40, 30, 5], 0.5, rng, batch_loss=px.SoftmaxCrossEntropyLoss())
+    static, state = px.NetworkBuilder.from_edges(net, n, frm, to, weights=w, input_ids=inputs, output_ids=outputs,
+                                                 device=cuda)
+    step = px.make_step(net, static, batch_size=64, device=cuda, activation_checkpoint="e4m3")
+    centres = rng.standard_normal((5, 16)) * 2
+    for _ in range(60):
+        label = rng.integers(0, 5, 64)
+        x = (centres[label] + rng.standard_normal((64, 16)) * 0.3).astype(np.float32)
+        step(state, px.StepInputs(x, np.eye(5, dtype=np.float32)[label]))
+    label = rng.integers(0, 5, 200)
+    x = (centres[label] + rng.standard_normal((200, 16)) * 0.3).astype(np.float32)
+    got = px.make_infer(net, static, state)(x).cpu().numpy().T
+    host = [{k: b[k].cpu().numpy() for k in ("from_id", "to_id", "dead", "weight")} for b in state.conns]
+    frm, to, w = (np.concatenate([b[k][b["dead"] == 0] for b in host]) for k in ("from_id", "to_id", "weight"))
+    level, held = state.units["level"].cpu().numpy(), w.astype(np.float64)
+    for u in range(n):
+        e = np.nonzero(to == u)[0]
+        if e.size:
+            held[e] = _mx.values(*_mx.quantize(w[e][None], "e2m1"), "e2m1", e.size)[0]
+    xt = x.T.astype(np.float64)
+    y4, err = _topological(level, frm, to, held, xt, inputs, outputs, "relu", "identity")
+    _within(got, y4[outputs], err[outputs] + 1e-30)
+    y, _ = _topological(level, frm, to, w.astype(np.float64), xt, inputs, outputs, "relu", "identity")
+    off = np.zeros_like(y)
+    for lv in range(1, int(level.max()) + 1):  # |w4 x4 - w x| <= |w4 - w| |x| + |w4| |x4 - x|, ReLU's slope at most 1
+        for u in np.nonzero(level == lv)[0]:
+            e = to == u
+            off[u] = (np.abs(held[e] - w[e])[:, None] * np.abs(y[frm[e]]) + np.abs(held[e])[:, None] * off[frm[e]]).sum(0)
+    bound = off[outputs] * 1.01 + err[outputs] + 1e-30
+    assert (np.abs(got - y[outputs]) <= bound).all()
+    order = np.sort(y[outputs], axis=0)
+    sure = order[-1] - order[-2] > 2 * bound.max(0)
+    assert np.array_equal(got.argmax(0)[sure], y[outputs].argmax(0)[sure])

@@ -20,11 +20,12 @@ made from them in place and, once the checkpoint has them, the backward's sums
 and gradients: 4 (rows) + 4 (the loss seeds) + 33/32 bytes a unit and sample
 instead of 16. A row serves all of these because an edge of a TOPOLOGICAL net
 goes to a deeper level and lies in the bucket of its source's level, so a
-level's sums are complete before its apply. The step checks that on a state's columns when it first sees them, and again once
-they were replaced or edited by torch operations (not through `.data` or
-another alias: such an edit needs a new column); the growth rule must have
-direction "deeper". The check reads the host, so a step is run once on a state
-before it is captured, and a captured step does not repeat it.
+level's sums are complete before its apply. The step checks that on a state's
+columns when it first sees them, and again once they were replaced or edited by
+torch operations (not through `.data` or another alias: such an edit needs a
+new column); the growth rule must have direction "deeper". The check reads the
+host, so a step is run once on a state before it is captured, and a captured
+step does not repeat it.
 """
 
 from __future__ import annotations

@@ -192,10 +192,15 @@ __device__ __forceinline__ void finish_slot(const EdgeGrad &k, int64_t s, bool l
 }
 
 // Every warp takes 32 slots at a time over the whole batch. What costs is the
-// gradient rows, 128 bytes a slot and slice. Rows that an L1 can hold in part
-// gain from it, and more warps an SM would only push them out; larger ones come
-// from L2 whatever the L1 does, and want the loads of a fourth block an SM
-// (MIN_BLOCKS).
+// gradient rows, 128 bytes a slot and slice, and a shuffle of their offset for
+// each load: over 2^22 slots of 65,536 units (128 samples, 119 us) the loads'
+// data pipe is 66 % busy, L1 71 %, L2 47 %, and warps wait for loads (7 of 12
+// cycles between issues) with 46 % of them resident: latency and that pipe, no
+// rate of a memory. MIN_BLOCKS: a warp reads one slice of its rows after
+// another, so what the rows' reuse in L1 depends on is the units, not the
+// batch. 2^19 slots with three and with four blocks an SM: 1,000 units and 128
+// samples 20.4 and 21.7 us, 2,794 and 256 36.0 and 37.7, 16,384 and 256 36.3 and
+// 35.7, 65,536 and 256 40.8 and 39.8 (8,192 units: alike).
 template <int FMT, bool VEC, bool WIDE, int MIN_BLOCKS>
 __global__ void __launch_bounds__(256, MIN_BLOCKS) mx_edge_grad_kernel(EdgeGrad k) {
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
@@ -232,14 +237,17 @@ __global__ void __launch_bounds__(256) mx_edge_grad_split_kernel(EdgeGrad k) {
 // Where the slots are a good part of all pairs of units, every pair's sum is a
 // matrix product, D[t, f] = sum_b g[t, b] * a[f, b], and the slots pick theirs
 // from it. With 256 samples, us so and slot by slot: 400 x 300 units and 2^20
-// slots 15 and 74, 1000 x 1000 and 2^19 30 and 37 (43 partly regrown), 1000 x
-// 1000 and 300,000 28 and 25. An 8-bit activation is a bfloat16 exactly (four
-// significant bits, a power of two), and a float32 gradient is the sum of three
-// bfloat16 (8 + 8 + 8 bits), so three tensor-core products, added in float32,
-// hold what the float32 products do. Only the 64 x 64 tiles that some slot
+// slots 14 and 74, 1000 x 1000 and 2^19 27 and 37 (43 partly regrown). An 8-bit
+// activation is a bfloat16 exactly (four significant bits, a power of two), and
+// a float32 gradient is the sum of three bfloat16 (8 + 8 + 8 bits), both down to
+// 2^-133, so three tensor-core products, added in float32, hold what the float32
+// products do but for parts below that. Only the 64 x 64 tiles that some slot
 // touches are computed; the product lies in the caller's scratch, n^2 floats,
-// in L2. mma.sync is the bound of the middle kernel (tensor pipes 30 % busy over
-// its two rounds of tiles); the launches around it cost as much again.
+// in L2. Latency bounds the middle kernel (18 us of the 27 under the profiler):
+// two barriers a 32-sample slice around one buffer, and every source tile
+// splits the gradient rows into their parts again (1.5 instructions a cycle,
+// 25 % of the warps, first stall shared memory, tensor pipes 30 % busy); the
+// launches around it cost as much again.
 constexpr int kPairTile = 64, kPairUnits = 4096, kPairSlots = 49152;
 
 __host__ __device__ inline int pair_tiles(uint32_t n) { return static_cast<int>((n + kPairTile - 1) / kPairTile); }
@@ -706,10 +714,13 @@ __device__ __forceinline__ void sum_scaled(const Conns &c, const Rows &r, const 
 // A warp takes a block of 32 edges of an item: lane j holds edge j's row and
 // weight, and fetches the next block's while this one's rows come. A row is
 // LANES pieces, so 32 / LANES edges are read side by side, each load
-// instruction full, two in flight a lane. The loop waits on L2 and issues about
-// three instructions a pair of samples (two conversions and a paired FMA, on
-// two pipes), so warps count for more than loads a warp: 64 registers, 32 warps
-// an SM.
+// instruction full, two in flight a lane. MX rows: the loop waits for loads and
+// issues about three instructions a pair of samples (two conversions and a
+// paired FMA, on two pipes), so warps count for more than loads a warp: 64
+// registers, 32 warps an SM (32,768 x 96 in-edges, 100 samples of e2m1, 89 us:
+// 2.7 instructions a cycle, ALU pipe 48 %, L2 22 %). Float32 rows: two loads in
+// flight a lane are the bound (256 samples, 343 us: 9.4 TB/s of rows, L2 40 %,
+// 14 cycles of waiting for loads between issues; a 1000 x 1000 pair, 19 us).
 template <int XF, int LANES, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(256, 4) mx_product_kernel(Conns c, Rows r, int act_kind, Out out, Items n) {
   using O = typename Offset<WIDE>::type;
@@ -902,7 +913,10 @@ __global__ void __launch_bounds__(256) mx_product_short_kernel(Conns c, Rows r, 
 
 // How many warps share a destination (`wpd`, up to a CTA's eight) and, past
 // that, CTAs: until every SM has 32 warps' worth or a warp has one block of 32
-// edges left.
+// edges left. By the mean in-degree: where the items fill the SMs, a destination
+// far above it is one warp's (or eight lanes') work from end to end. 32,768
+// destinations of 64 in-edges, one of them with 0 / 4,096 / 65,536 more: one
+// float32 sample 12 / 54 / 690 us, 64 samples of e2m1 49 / 156 / 1,980 us.
 static void split_items(int64_t items, int64_t mean, int *wpd, int *ranks) {
   const int64_t warps = static_cast<int64_t>(sm_count()) * 32;
   *wpd = *ranks = 1;
@@ -966,8 +980,11 @@ static int launch_product(const Conns &c, const Rows &r, int act, const Out &out
 }
 
 // Scratch of the pair product (0 where slot by slot is as good): the pairs'
-// sums, then a bit a tile. At a twelfth of all pairs of units (between two
-// levels of a layered net a third or more of theirs) the two are alike; and
+// sums, then a bit a tile. At a twelfth of all pairs of units the two are alike
+// (300,000 slots of 2,000 units: 25 us each). The pairs are those of all the
+// net's units, not of the levels that a bucket joins, so a deeper net's bucket
+// stays slot by slot although its own level pair is as full (2^19 slots of 1000
+// x 1000 units: 27 us in a net of 2,000 units, 37 in one of 2,794); and
 // enough work to pay for four launches. A tile is one CTA over the whole batch,
 // so a small net's long batch is few CTAs' work however many slots it has, and
 // the slots have to be worth that: 64 units, 4,096 samples, slot by slot and so:

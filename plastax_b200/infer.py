@@ -10,9 +10,9 @@ float32, the values the training step's forward leaves in the output units
 0 and no input, or pruned) keeps its activation: the state's, as the streaming
 step reads it, or 0 for a net with a `batch_reduction`, whose batched step
 starts from rows of zeros. A ReLU keeps what is not a number, which the step's
-makes 0. One kernel a level does the product, the
-activation and, with `rows` an MX format, the quantisation of the level's rows
-for the next one; the outputs are always float32.
+makes 0. One kernel a level does the product, the activation and, with `rows`
+an MX format, the quantisation of the level's rows for the next one; the
+outputs are always float32.
 
 The layout is a snapshot (of those activations too): later steps on `state` do
 not change it.

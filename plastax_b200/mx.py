@@ -326,7 +326,9 @@ class MxConns:
     (`weight`, one an edge) or an MX format, in blocks of 32 consecutive
     in-edges of one destination: blocks [block_offsets[i], block_offsets[i +
     1]) of `codes` (uint8 [blocks, 32], e2m1 [blocks, 16]) and `scales` (uint8
-    [blocks]). Offsets are int64."""
+    [blocks]). Offsets are int64. The tensors' memory is taken when the
+    connections are made: values may be edited in place, but a tensor that gets
+    other memory (`set_`, `.data`) needs new connections."""
 
     units: torch.Tensor
     offsets: torch.Tensor
